@@ -314,6 +314,150 @@ int pspml_model_fail_next(pspml_model* m, int32_t count, int32_t status);
 int pspml_forward_timed(pspml_model* m, const int8_t* dev_in, int8_t* dev_out,
                         int64_t batch, float* ms_per_op, void* stream);
 
+/* ------------------------------------------------- attention (serving)
+ * What an autoregressive network needs between its projections (which run
+ * on the fully connected calls above): rotary positions, a paged cache of
+ * keys and values, and attention over whole prompts and over the cache.  No
+ * counterpart in the reference.  Device pointers except where a comment says
+ * "host"; asynchronous on `stream`.
+ *
+ * Calls of one context that use its workspace (pspml_attention_cached and
+ * pspml_attention_prompt) are ordered after one another by the library when
+ * they are given different streams.  Under stream capture that ordering is
+ * the caller's: replays of graphs that share a context run one at a time. */
+typedef enum pspml_dtype {
+  PSPML_DTYPE_F32 = 0,
+  PSPML_DTYPE_F16 = 1,
+  PSPML_DTYPE_BF16 = 2,
+  PSPML_DTYPE_S8 = 3  /* value = scale * (q - zero_point)                   */
+} pspml_dtype;
+
+/* A [tokens][heads][head_dim] view.  Strides count elements; a head's
+ * elements are contiguous.  scale and zero_point are read for PSPML_DTYPE_S8
+ * only.  Outputs may not overlap inputs, except that pspml_rotary_* accept
+ * q_out and k_out that are exactly the view of q and k. */
+typedef struct pspml_heads {
+  void* data;
+  int64_t token_stride, head_stride;
+  int32_t heads, head_dim;
+  int32_t dtype;
+  int32_t zero_point;
+  float scale;
+  int32_t reserved;      /* 0 */
+} pspml_heads;
+
+/* Key and value pools of `pages` pages of page_size slots; both pools have
+ * the strides given (elements; a head's elements are contiguous), so a page
+ * may hold [slot][head][dim] or [head][slot][dim].  dtype is F32, F16 or
+ * BF16. */
+typedef struct pspml_kv_cache {
+  void* k;
+  void* v;
+  int64_t page_stride, slot_stride, head_stride;
+  int64_t pages;
+  int32_t page_size;
+  int32_t heads, head_dim;
+  int32_t dtype;
+} pspml_kv_cache;
+
+/* Rotary positions.  Pair i < rot_dim/2 of a head turns by position * f_i:
+ * f_i = base^(-2i/rot_dim), scaled for contexts longer than the trained one:
+ *   NONE    f_i
+ *   LINEAR  f_i / factor
+ *   BASE    base * factor^(rot_dim/(rot_dim-2)) in place of base
+ *   PARTS   with r_i = original_len * f_i / 2pi turns over the trained
+ *           length: f_i where r_i >= high, f_i / factor where r_i <= low,
+ *           and a mix even in r_i between.
+ * HALF pairs element i with i + rot_dim/2, INTERLEAVED 2i with 2i + 1;
+ * elements from rot_dim on pass through.  rot_dim 0 rotates nothing.
+ * amplitude multiplies the rotated elements. */
+#define PSPML_ROTARY_HALF 0
+#define PSPML_ROTARY_INTERLEAVED 1
+#define PSPML_ROTARY_SCALE_NONE 0
+#define PSPML_ROTARY_SCALE_LINEAR 1
+#define PSPML_ROTARY_SCALE_BASE 2
+#define PSPML_ROTARY_SCALE_PARTS 3
+typedef struct pspml_rotary_desc {
+  int32_t head_dim;      /* 1 .. 1024                                       */
+  int32_t rot_dim;       /* even, 0 .. head_dim                             */
+  int32_t layout;        /* PSPML_ROTARY_HALF / _INTERLEAVED                */
+  int32_t scaling;       /* PSPML_ROTARY_SCALE_*                            */
+  double base;
+  double factor;
+  double low, high;      /* PARTS                                           */
+  double original_len;   /* PARTS                                           */
+  double amplitude;
+} pspml_rotary_desc;
+typedef struct pspml_rotary pspml_rotary;
+
+/* Writes the rot_dim/2 frequencies to host memory, in turns per position as
+ * 64-bit binary fractions (f_i / 2pi * 2^64, modulo a turn): a position
+ * times a frequency wraps exactly, so angles lose nothing at any position.
+ * Needs no device. */
+int pspml_rotary_frequencies(const pspml_rotary_desc* d, uint64_t* host_out);
+/* A rotation kept on the context's device. */
+int pspml_rotary_create(pspml_ctx* ctx, const pspml_rotary_desc* d, pspml_rotary** out);
+int pspml_rotary_destroy(pspml_rotary* r);
+
+/* Rotates q into q_out and, when k is given (k and k_out may both be NULL),
+ * k into k_out.  positions [tokens] int32.  Inputs F32, F16, BF16 or S8;
+ * outputs F32, F16 or BF16; q and k have one dtype, their outputs one. */
+int pspml_rotary_apply(pspml_rotary* r, int64_t tokens, const int32_t* positions,
+                       const pspml_heads* q, const pspml_heads* q_out, const pspml_heads* k,
+                       const pspml_heads* k_out, void* stream);
+
+/* pspml_rotary_apply of q into q_out (both may be NULL), of k into the
+ * cache, and the copy of v to the cache.  Token t goes to slot slots[t] =
+ * page * page_size + slot; a slot outside the cache is skipped.  Two tokens
+ * may not name one slot. */
+int pspml_rotary_append(pspml_rotary* r, int64_t tokens, const int32_t* positions,
+                        const int64_t* slots, const pspml_heads* q, const pspml_heads* q_out,
+                        const pspml_heads* k, const pspml_heads* v, const pspml_kv_cache* cache,
+                        void* stream);
+
+/* Row at position p of its sequence sees the keys j of that sequence with
+ * j <= p (causal) and j > p - window (window > 0, needs causal), weighted
+ * by softmax(scale * q.k).  A row that sees no key gives zeros and a
+ * log-sum-exp of -inf.  Keys past a sequence's end never count, whatever
+ * their slots hold; a non-finite value of a sequence's own key may reach any
+ * of that sequence's rows. */
+typedef struct pspml_attention_desc {
+  float scale;
+  int32_t causal;        /* 0 / 1                                           */
+  int32_t window;        /* 0: none                                         */
+  int32_t reserved;      /* 0 */
+} pspml_attention_desc;
+
+/* Attention over packed whole prompts.  q, k, v and out hold `tokens`
+ * tokens; sequence s is tokens starts[s] .. starts[s+1] (int32, sequences
+ * + 1 of them, not decreasing).  Tokens of no sequence are not written.
+ * q->heads is a multiple of k->heads.  q, k, v have one dtype of F32, F16,
+ * BF16; out has the same one or S8 (rounded to nearest, ties to even, and
+ * clamped).  lse: NULL or [tokens][q->heads] float, natural logarithm.
+ * head_dim <= 256.  Tensor cores take F16 and BF16 of head_dim <= 128,
+ * a multiple of 8, at 16-byte aligned bases and strides; anything else runs
+ * on CUDA cores. */
+int pspml_attention_prompt(pspml_ctx* ctx, const pspml_attention_desc* d, int64_t tokens,
+                           int32_t sequences, const int32_t* starts, const pspml_heads* q,
+                           const pspml_heads* k, const pspml_heads* v, const pspml_heads* out,
+                           float* lse, void* stream);
+
+/* Attention of new tokens over the cache, which holds them too (append
+ * first).  Sequence s has the new tokens starts[s] .. starts[s+1] of q, at
+ * most max_new (a host-side bound; rows past it are not computed), and
+ * lengths[s] keys in all, so its row r sits at position
+ * lengths[s] - (starts[s+1] - starts[s]) + r.  Its keys are in the pages
+ * pages[s * pages_stride + i], i < ceil(lengths[s] / page_size) (int32;
+ * entries past that are not read; lengths past pages_stride pages are cut
+ * there).  A page outside the pool reads as zeros.  Types as
+ * pspml_attention_prompt, with the cache's dtype equal to q's; the tensor
+ * cores also need page_size a multiple of 8. */
+int pspml_attention_cached(pspml_ctx* ctx, const pspml_attention_desc* d, int64_t tokens,
+                           int32_t sequences, int32_t max_new, const int32_t* starts,
+                           const int32_t* lengths, const int32_t* pages, int64_t pages_stride,
+                           const pspml_heads* q, const pspml_kv_cache* cache,
+                           const pspml_heads* out, float* lse, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -41,6 +41,20 @@ OP_RESHAPE = 6
 F32_RELU = 1
 F32_GEMM_ORDER = 2
 
+# pspml_dtype
+DTYPE_F32 = 0
+DTYPE_F16 = 1
+DTYPE_BF16 = 2
+DTYPE_S8 = 3
+
+# pspml_rotary_desc layouts and scalings
+ROTARY_HALF = 0
+ROTARY_INTERLEAVED = 1
+ROTARY_SCALE_NONE = 0
+ROTARY_SCALE_LINEAR = 1
+ROTARY_SCALE_BASE = 2
+ROTARY_SCALE_PARTS = 3
+
 # Byte-for-byte layout of struct pspml_op_desc.
 OP_DESC_FIELDS_I32 = (
     "kind", "in_h", "in_w", "in_c", "out_h", "out_w", "out_c",
@@ -66,6 +80,39 @@ class Timing(ctypes.Structure):
     _fields_ = [("total_ms", ctypes.c_double), ("h2d_bytes", ctypes.c_double),
                 ("d2h_bytes", ctypes.c_double), ("micro_batches", ctypes.c_int32),
                 ("devices", ctypes.c_int32), ("rerun_shards", ctypes.c_int32)]
+
+
+class Heads(ctypes.Structure):
+    """struct pspml_heads: a [tokens][heads][head_dim] view."""
+    _fields_ = [("data", ctypes.c_void_p), ("token_stride", ctypes.c_int64),
+                ("head_stride", ctypes.c_int64), ("heads", ctypes.c_int32),
+                ("head_dim", ctypes.c_int32), ("dtype", ctypes.c_int32),
+                ("zero_point", ctypes.c_int32), ("scale", ctypes.c_float),
+                ("reserved", ctypes.c_int32)]
+
+
+class KvCacheView(ctypes.Structure):
+    """struct pspml_kv_cache: paged key and value pools."""
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("page_stride", ctypes.c_int64),
+                ("slot_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64),
+                ("pages", ctypes.c_int64), ("page_size", ctypes.c_int32),
+                ("heads", ctypes.c_int32), ("head_dim", ctypes.c_int32),
+                ("dtype", ctypes.c_int32)]
+
+
+class RotaryDesc(ctypes.Structure):
+    """struct pspml_rotary_desc."""
+    _fields_ = [("head_dim", ctypes.c_int32), ("rot_dim", ctypes.c_int32),
+                ("layout", ctypes.c_int32), ("scaling", ctypes.c_int32),
+                ("base", ctypes.c_double), ("factor", ctypes.c_double),
+                ("low", ctypes.c_double), ("high", ctypes.c_double),
+                ("original_len", ctypes.c_double), ("amplitude", ctypes.c_double)]
+
+
+class AttentionDesc(ctypes.Structure):
+    """struct pspml_attention_desc."""
+    _fields_ = [("scale", ctypes.c_float), ("causal", ctypes.c_int32),
+                ("window", ctypes.c_int32), ("reserved", ctypes.c_int32)]
 
 
 class PspmlError(RuntimeError):
@@ -116,6 +163,15 @@ _PROTOS = {
                                              ctypes.POINTER(Timing)]),
     "pspml_forward_timed": (ctypes.c_int, [_vp, _vp, _vp, _i64, ctypes.POINTER(ctypes.c_float),
                                            _vp]),
+    "pspml_rotary_frequencies": (ctypes.c_int, [_vp, _vp]),
+    "pspml_rotary_create": (ctypes.c_int, [_vp, _vp, ctypes.POINTER(_vp)]),
+    "pspml_rotary_destroy": (ctypes.c_int, [_vp]),
+    "pspml_rotary_apply": (ctypes.c_int, [_vp, _i64, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "pspml_rotary_append": (ctypes.c_int, [_vp, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "pspml_attention_prompt": (ctypes.c_int, [_vp, _vp, _i64, _i32, _vp, _vp, _vp, _vp, _vp,
+                                              _vp, _vp]),
+    "pspml_attention_cached": (ctypes.c_int, [_vp, _vp, _i64, _i32, _i32, _vp, _vp, _vp, _i64,
+                                              _vp, _vp, _vp, _vp, _vp]),
 }
 
 _lib = None
