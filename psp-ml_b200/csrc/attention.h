@@ -8,6 +8,7 @@
 #include <cstdint>
 
 #include "../../include/pspml.h"
+#include "runtime.h"
 
 struct pspml_rotary {
   pspml_ctx* ctx = nullptr;
@@ -113,7 +114,18 @@ struct RotaryArgs {
   float scale, amplitude;
 };
 
+// What a split call may use between its CTAs.
+struct AttnWork {
+  uint8_t* base;        // workspace
+  size_t bytes;
+  unsigned* counters;   // kAttnCounters words, zero between calls
+  unsigned* err;        // the context's device error word
+  int num_sms;
+};
+
 cudaError_t launch_rotary(const RotaryArgs& a, int num_sms, cudaStream_t s);
 cudaError_t launch_attn_any(const AttnArgs& a, cudaStream_t s);
+cudaError_t launch_attn_step(const AttnArgs& a, const AttnWork& w, cudaStream_t s);
+cudaError_t launch_attn_tc(const AttnArgs& a, const AttnWork& w, cudaStream_t s);
 
 }  // namespace pspml

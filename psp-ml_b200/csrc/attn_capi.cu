@@ -237,7 +237,52 @@ void fill_attention(const pspml_attention_desc* d, int64_t tokens, int32_t seque
   a->out_zero = out->dtype == PSPML_DTYPE_S8 ? out->zero_point : 0;
 }
 
+bool aligned(const void* p, int64_t bytes) {
+  return reinterpret_cast<uintptr_t>(p) % static_cast<uintptr_t>(bytes) == 0;
+}
+
+// What the tensor-core kernels' 16-byte loads and 8-element stores need.
+bool vector_form(const AttnArgs& a) {
+  if (a.dtype == PSPML_DTYPE_F32 || a.dim > 128 || a.dim % 8 != 0) return false;
+  const int out_bytes = a.out_dtype == PSPML_DTYPE_S8 ? 8 : 16;
+  return aligned(a.q, 16) && aligned(a.k, 16) && aligned(a.v, 16) && aligned(a.out, out_bytes) &&
+         (a.q_token | a.q_head | a.kv_token | a.kv_head | a.v_token | a.v_head | a.page_stride |
+          a.o_token | a.o_head) % 8 == 0;
+}
+
+// Calls that use the workspace run one after another even when they are
+// given different streams.  Under capture an event of the outside cannot be
+// waited for: there the caller keeps the order.
+int with_workspace(pspml_ctx* ctx, const AttnArgs& a, cudaStream_t s,
+                   cudaError_t (*launch)(const AttnArgs&, const AttnWork&, cudaStream_t)) {
+  AttnWork w;
+  w.base = ctx->workspace;
+  w.bytes = ctx->workspace_bytes;
+  w.counters = ctx->dev_err + 64;
+  w.err = ctx->dev_err;
+  w.num_sms = ctx->num_sms;
+  cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+  int st = cuda_status(cudaStreamIsCapturing(s, &capture), "cudaStreamIsCapturing");
+  if (st) return st;
+  const bool order = capture == cudaStreamCaptureStatusNone;
+  if (order && ctx->attn_used && ctx->attn_stream != s &&
+      (st = cuda_status(cudaStreamWaitEvent(s, ctx->attn_done, 0), "cudaStreamWaitEvent")))
+    return st;
+  if ((st = cuda_status(launch(a, w, s), "attention launch"))) return st;
+  if (order) {
+    if ((st = cuda_status(cudaEventRecord(ctx->attn_done, s), "cudaEventRecord"))) return st;
+    ctx->attn_used = true;
+    ctx->attn_stream = s;
+  }
+  return PSPML_OK;
+}
+
+// Few rows a key head: the cache's bytes bound the call (attn_step.cu);
+// anything the vector form does not fit: attn_any.cu.
 int run_attention(pspml_ctx* ctx, const AttnArgs& a, cudaStream_t s) {
+  if (!vector_form(a)) return cuda_status(launch_attn_any(a, s), "attention launch");
+  const int64_t group = a.q_heads / a.kv_heads;
+  if (a.paged && a.max_new * group <= 16) return with_workspace(ctx, a, s, launch_attn_step);
   return cuda_status(launch_attn_any(a, s), "attention launch");
 }
 

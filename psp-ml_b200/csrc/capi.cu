@@ -228,16 +228,19 @@ int pspml_ctx_create(int device, size_t workspace_bytes, pspml_ctx** out) {
   ctx->device = device;
   ctx->num_sms = prop.multiProcessorCount;
   ctx->workspace_bytes = workspace_bytes ? workspace_bytes : (64u << 20);
-  st = cuda_status(cudaMalloc(&ctx->dev_err, 256), "cudaMalloc(error word)");
+  st = cuda_status(cudaMalloc(&ctx->dev_err, kDevErrBytes), "cudaMalloc(error word)");
   if (!st)
     st = cuda_status(cudaMalloc(&ctx->workspace, ctx->workspace_bytes), "cudaMalloc(workspace)");
   if (!st)
     st = cuda_status(cudaStreamCreateWithFlags(&ctx->stream, cudaStreamNonBlocking),
                      "cudaStreamCreate");
+  if (!st)
+    st = cuda_status(cudaEventCreateWithFlags(&ctx->attn_done, cudaEventDisableTiming),
+                     "cudaEventCreate");
   // Cleared on the context's own stream and waited for: a plain cudaMemset
   // runs on the legacy default stream, which non-blocking streams do not
   // wait for.
-  if (!st) st = cuda_status(cudaMemsetAsync(ctx->dev_err, 0, 256, ctx->stream), "cudaMemset");
+  if (!st) st = cuda_status(cudaMemsetAsync(ctx->dev_err, 0, kDevErrBytes, ctx->stream), "cudaMemset");
   if (!st) st = cuda_status(cudaStreamSynchronize(ctx->stream), "cudaMemset");
   if (st) {
     pspml_ctx_destroy(ctx);
@@ -251,6 +254,7 @@ int pspml_ctx_destroy(pspml_ctx* ctx) {
   if (ctx == nullptr) return PSPML_OK;
   cudaSetDevice(ctx->device);
   if (ctx->stream) cudaStreamDestroy(ctx->stream);
+  if (ctx->attn_done) cudaEventDestroy(ctx->attn_done);
   if (ctx->workspace) cudaFree(ctx->workspace);
   if (ctx->dev_err) cudaFree(ctx->dev_err);
   delete ctx;
@@ -271,7 +275,8 @@ int pspml_ctx_check_device(pspml_ctx* ctx) {
                        "read device error word");
   if (st) return st;
   if (v != 0) {
-    cudaMemsetAsync(ctx->dev_err, 0, sizeof(unsigned), ctx->stream);
+    // The counters too: a kernel that gave up may have left one part-way.
+    cudaMemsetAsync(ctx->dev_err, 0, kDevErrBytes, ctx->stream);
     cudaStreamSynchronize(ctx->stream);
     char buf[96];
     std::snprintf(buf, sizeof(buf), "a kernel gave up on a bounded wait (code %u)", v);

@@ -12,14 +12,23 @@
 #include "../../include/pspml.h"
 #include "kernels.h"
 
+// Arrival counters of split attention calls, after the error word's 256 bytes.
+constexpr int kAttnCounters = 1024;
+constexpr size_t kDevErrBytes = 256 + kAttnCounters * sizeof(unsigned);
+
 struct pspml_ctx {
   int device = 0;
   int num_sms = 148;
   int64_t timeout_ms = 0;
-  unsigned* dev_err = nullptr;      // device error word written by kernels
+  unsigned* dev_err = nullptr;      // device error word written by kernels, attention counters
   uint8_t* workspace = nullptr;     // per-op prepared tables (folded bias, requant)
   size_t workspace_bytes = 0;
   cudaStream_t stream = nullptr;    // internal stream for synchronous work
+  // Last attention call that used the workspace: a call on another stream
+  // waits for it.
+  cudaEvent_t attn_done = nullptr;
+  cudaStream_t attn_stream = nullptr;
+  bool attn_used = false;
 };
 
 namespace pspml {
