@@ -126,6 +126,7 @@ struct AttnWork {
 cudaError_t launch_rotary(const RotaryArgs& a, int num_sms, cudaStream_t s);
 cudaError_t launch_attn_any(const AttnArgs& a, cudaStream_t s);
 cudaError_t launch_attn_step(const AttnArgs& a, const AttnWork& w, cudaStream_t s);
+bool attn_tc_covers(const AttnArgs& a);
 cudaError_t launch_attn_tc(const AttnArgs& a, const AttnWork& w, cudaStream_t s);
 
 }  // namespace pspml

@@ -151,7 +151,8 @@ int check_rotary_pair(const pspml_rotary* r, const pspml_heads* in, const pspml_
   if (st) return st;
   if (in->head_dim != r->d.head_dim) return bad(n + ": head_dim differs from the rotary's");
   if (out == nullptr) return PSPML_OK;
-  if ((st = check_heads(out, (n + " output").c_str(), tokens, true))) return st;
+  st = check_heads(out, (n + " output").c_str(), tokens, true);
+  if (st) return st;
   if (out->dtype == PSPML_DTYPE_S8) return bad(n + " output: S8 is not an output type here");
   if (out->heads != in->heads || out->head_dim != in->head_dim)
     return bad(n + ": input and output shapes differ");
@@ -277,12 +278,13 @@ int with_workspace(pspml_ctx* ctx, const AttnArgs& a, cudaStream_t s,
   return PSPML_OK;
 }
 
-// Few rows a key head: the cache's bytes bound the call (attn_step.cu);
-// anything the vector form does not fit: attn_any.cu.
+// Few rows a key head: the cache's bytes bound the call (attn_step.cu); more
+// rows: attn_tc.cu; what neither fits: attn_any.cu.
 int run_attention(pspml_ctx* ctx, const AttnArgs& a, cudaStream_t s) {
   if (!vector_form(a)) return cuda_status(launch_attn_any(a, s), "attention launch");
   const int64_t group = a.q_heads / a.kv_heads;
   if (a.paged && a.max_new * group <= 16) return with_workspace(ctx, a, s, launch_attn_step);
+  if (attn_tc_covers(a)) return with_workspace(ctx, a, s, launch_attn_tc);
   return cuda_status(launch_attn_any(a, s), "attention launch");
 }
 

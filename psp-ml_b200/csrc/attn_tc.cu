@@ -1,0 +1,705 @@
+// attn_tc.cu - attention over whole prompts and of chunks of new tokens over
+// the paged cache on the tensor cores (tcgen05), F16 and BF16.
+//
+//   S = Q K^T,  P = exp2(c S - m),  O = P V / sum P,   c = scale * log2 e
+//
+// Rows of a tile are (token, head of the key head's group) pairs, 128 / group
+// tokens a tile: the heads that share keys share their loads, short chunks
+// fill a tile with heads, and the causal edge is a few tokens wide instead
+// of 128.  A CTA takes two such tiles (A, B) against one stream of 128-key
+// tiles, so that the tensor cores work on one tile while the softmax of the
+// other runs:
+//   warps 0-3, 4-7  softmax of A and B, one row per thread: S from tensor
+//                   memory, running maximum and sum in registers, P back to
+//                   tensor memory over S (as the A operand of P V); the
+//                   output is rescaled only when the maximum has grown by
+//                   more than 2^8 since the last time, by the same threads
+//   warp 8          TMA loads: Q once, K and V tiles through a ring of slots
+//   warp 9          (10 and 11 idle) one thread issues the MMAs: P V of a tile, then the next
+//                   Q K^T of the same tile once P has been read
+// Tensor memory: S/P of A and B (128 columns each), O of A and B.
+//
+// Keys that no row of the CTA sees are not loaded; the values between such a
+// key and the 16-key step of the P V product that holds it are zeroed in
+// shared memory, since 0 * NaN would spread whatever they hold.  Heads of
+// fewer than DP elements are padded with zeros by TMA.
+//
+// With few tiles the keys of each are cut into equal parts for several CTAs;
+// the unnormalised parts go to the workspace and the CTA that arrives last
+// joins them in order.
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <atomic>
+#include <cmath>
+#include <type_traits>
+
+#include "attention.h"
+#include "ptx.cuh"
+
+namespace pspml {
+
+CUresult encode_tensor_map(CUtensorMap* map, const void* base, int rank, const uint64_t* dims,
+                           const uint64_t* strides_bytes, const uint32_t* box,
+                           const uint32_t* elem_strides, CUtensorMapSwizzle swizzle);
+
+namespace {
+
+// Three warpgroups: 168 registers a thread at launch, of which the softmax
+// groups take 208 and the third keeps 88 (128 * (2 * 208 + 88) = 384 * 168).
+constexpr int kTcThreads = 384;
+constexpr int kSoftmaxRegs = 208;
+constexpr int kOtherRegs = 88;
+constexpr int kTcWarps = kTcThreads / 32;
+constexpr int kKeys = 128;        // keys a tile
+constexpr float kGrowLog2 = 8.0f; // largest stale maximum, as a power of two
+
+struct TcArgs {
+  AttnArgs a;
+  float* part_o;       // [ctas][256][DP]
+  float2* part_ml;     // [ctas][256]
+  unsigned* arrived;   // [segments]
+  unsigned* err;
+  float scale_log2;
+  int32_t group, tile_tokens, splits, box_keys;
+};
+
+template <int DP>
+struct TcShape {
+  static constexpr int kHalves = DP / 64;           // 128-byte swizzled halves of a row
+  static constexpr int kTileBytes = 128 * DP * 2;   // Q tile, K or V slot
+  static constexpr int kSlots = DP == 128 ? 5 : 8;
+  static constexpr int kSmem = 1024 + (2 + kSlots) * kTileBytes;
+  static constexpr uint32_t kCols = DP == 128 ? 512 : 512;
+  static constexpr uint32_t kS = 0;                 // S/P of A, then of B
+  static constexpr uint32_t kO = 256;               // O of A, then of B
+};
+
+__device__ __forceinline__ float tc_ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ void tc_fail(unsigned* err, volatile int* abort, unsigned code) {
+  *abort = 1;
+  atomicCAS(err, 0u, code);
+}
+
+// Eight neighbouring outputs of a row.
+template <typename T>
+__device__ __forceinline__ void store8(const AttnArgs& a, int64_t at, const float* v) {
+  if (a.out_dtype == PSPML_DTYPE_S8) {
+    uint32_t w[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      w[i] = 0;
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        w[i] |= static_cast<uint32_t>(static_cast<uint8_t>(
+                    quantise_s8(v[4 * i + k], a.out_inv_scale, a.out_zero)))
+                << (8 * k);
+    }
+    *reinterpret_cast<uint2*>(static_cast<int8_t*>(a.out) + at) = make_uint2(w[0], w[1]);
+  } else {
+    *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + at) =
+        make_uint4(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]), pack2<T>(v[4], v[5]),
+                   pack2<T>(v[6], v[7]));
+  }
+}
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(kTcThreads, 1)
+    k_attn_tc(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+              const __grid_constant__ CUtensorMap map_v, const TcArgs p) {
+  using Sh = TcShape<DP>;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ uint64_t q_full, landed, s_full[2], p_full[2], o_done[2], drain;
+  __shared__ uint64_t kv_full[Sh::kSlots], kv_empty[Sh::kSlots];
+  __shared__ uint32_t tmem_slot;
+  __shared__ int abort_word;
+  __shared__ int64_t s_sum[kTcWarps];
+  __shared__ int s_seq;
+  __shared__ int64_t s_pair;
+  __shared__ int s_last;
+  const AttnArgs& a = p.a;
+  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
+  volatile int* abort = &abort_word;
+  uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
+  uint8_t* sq = smem;
+  uint8_t* slots = smem + 2 * Sh::kTileBytes;
+
+  // The CTA's pair of tiles: pairs are counted from the last sequence's last
+  // tokens, so that the pairs with the most keys come first.
+  const int pair_tokens = 2 * p.tile_tokens;
+  auto pairs_of = [&](const SeqSpan& sp) {
+    const int64_t rows = a.paged && sp.rows > a.max_new ? a.max_new : sp.rows;
+    return (rows + pair_tokens - 1) / pair_tokens;
+  };
+  const int per = (a.sequences + kTcThreads - 1) / kTcThreads;
+  const int f0 = min(a.sequences, tid * per), f1 = min(a.sequences, f0 + per);
+  int64_t mine = 0;
+  for (int s = f0; s < f1; ++s) mine += pairs_of(seq_span(a, s));
+  int64_t scan = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o *= 2) {
+    const int64_t v = __shfl_up_sync(~0u, scan, o);
+    if (lane >= o) scan += v;
+  }
+  if (lane == 31) s_sum[warp] = scan;
+  __syncthreads();
+  int64_t total = 0, before = scan - mine;
+#pragma unroll
+  for (int w = 0; w < kTcWarps; ++w) {
+    if (w < warp) before += s_sum[w];
+    total += s_sum[w];
+  }
+  const int part = static_cast<int>(blockIdx.x % p.splits);
+  const int64_t seg = blockIdx.x / p.splits;
+  const int head = static_cast<int>(seg % a.kv_heads);
+  const int64_t pair = total - 1 - seg / a.kv_heads;
+  if (pair < 0) return;
+  if (pair >= before && pair < before + mine) {
+    int64_t at = before;
+    int s = f0;
+    while (true) {
+      const int64_t n = pairs_of(seq_span(a, s));
+      if (pair < at + n) break;
+      at += n;
+      ++s;
+    }
+    s_seq = s;
+    s_pair = pair - at;
+  }
+  if (tid == 0) {
+    abort_word = 0;
+    mbar_init(&q_full, 1);
+    mbar_init(&landed, 1);
+    mbar_init(&drain, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_full[i], 4);
+      mbar_init(&o_done[i], 1);
+    }
+    for (int i = 0; i < Sh::kSlots; ++i) {
+      mbar_init(&kv_full[i], 1);
+      mbar_init(&kv_empty[i], 1);
+    }
+    fence_mbar_init();
+  }
+  if (warp == 8) {
+    tmem_alloc(&tmem_slot, Sh::kCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_slot;
+
+  // Rows, positions and keys of the two tiles.
+  const int seq = s_seq;
+  const SeqSpan sp = seq_span(a, seq);
+  const int64_t rows_all = a.paged && sp.rows > a.max_new ? a.max_new : sp.rows;
+  const int64_t tok0 = s_pair * pair_tokens;
+  const int64_t place0 = sp.keys - sp.rows + tok0;
+  const int64_t left = rows_all - tok0;  // at least 1
+  int tokens[2];
+  tokens[0] = static_cast<int>(left < p.tile_tokens ? left : p.tile_tokens);
+  tokens[1] = static_cast<int>(left < pair_tokens ? left : pair_tokens) - tokens[0];
+  int64_t lo = 0;
+  if (a.window > 0 && place0 - a.window + 1 > 0) lo = place0 - a.window + 1;
+  const int64_t start = lo / kKeys * kKeys;
+  int64_t hi[2];
+  int tiles[2];
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    hi[t] = sp.keys;
+    const int64_t end = place0 + t * p.tile_tokens + tokens[t];
+    if (a.causal && end < hi[t]) hi[t] = end;
+    tiles[t] = tokens[t] > 0 && hi[t] > lo ? static_cast<int>((hi[t] - start + kKeys - 1) / kKeys)
+                                           : 0;
+  }
+  const int64_t hi_all = tokens[1] > 0 ? hi[1] : hi[0];
+  const int n_all = tiles[0] > tiles[1] ? tiles[0] : tiles[1];
+  const int j0 = static_cast<int>(static_cast<int64_t>(n_all) * part / p.splits);
+  const int j1 = static_cast<int>(static_cast<int64_t>(n_all) * (part + 1) / p.splits);
+  const int n0 = max(0, min(j1, tiles[0]) - j0), n1 = max(0, min(j1, tiles[1]) - j0);
+  const int n = max(n0, n1);  // key tiles of this CTA
+  // Keys of tile j that some row sees: [v_lo, v_hi) of its 128.
+  auto v_lo = [&](int j) {
+    const int64_t x = lo - (start + static_cast<int64_t>(j) * kKeys);
+    return x > 0 ? static_cast<int>(x) : 0;
+  };
+  auto v_hi = [&](int j) {
+    const int64_t x = hi_all - (start + static_cast<int64_t>(j) * kKeys);
+    return x < kKeys ? static_cast<int>(x) : kKeys;
+  };
+
+  if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+  if (warp == 8) {
+    // ---------------------------------------------------------- TMA loads
+    const int boxes = kKeys / p.box_keys;  // one per lane
+    const int32_t* table = a.paged ? a.pages + seq * a.pages_stride : nullptr;
+    auto page_of = [&](int j) -> int {
+      const int64_t key = start + static_cast<int64_t>(j) * kKeys + lane * p.box_keys;
+      if (!a.paged || lane >= boxes || key < 0 || key + p.box_keys <= lo || key >= hi_all) return -1;
+      return table[key / a.page_size];
+    };
+    if (n > 0 && lane == 0) {
+      const int active = (n0 > 0) + (n1 > 0);
+      mbar_arrive_expect_tx(
+          &q_full, static_cast<uint32_t>(active * Sh::kHalves * p.tile_tokens * p.group * 128));
+      for (int t = 0; t < 2; ++t) {
+        if ((t == 0 ? n0 : n1) == 0) continue;
+        for (int h = 0; h < Sh::kHalves; ++h)
+          tma_load_4d(sq + t * Sh::kTileBytes + h * 16384, &map_q, &q_full, h * 128, 0, head,
+                      static_cast<int32_t>(sp.begin + tok0 + t * p.tile_tokens));
+      }
+    }
+    int slot = 0, landings = 0;
+    uint32_t phase = 0;
+    int issued = 0;
+    bool ok = true;
+    int page = n > 0 ? page_of(j0) : -1;
+    for (int j = j0; j < j0 + n && ok; ++j) {
+      const int64_t kb = start + static_cast<int64_t>(j) * kKeys;
+      const int lo_k = v_lo(j), hi_k = v_hi(j);
+      const int first = lane * p.box_keys;
+      const bool load = lane < boxes && first < hi_k && first + p.box_keys > lo_k;
+      const int n_load = __popc(__ballot_sync(~0u, load));
+      const uint32_t bytes = static_cast<uint32_t>(n_load * p.box_keys * 128 * Sh::kHalves);
+      const int next_page = j + 1 < j0 + n ? page_of(j + 1) : -1;
+      const int32_t c2 = a.paged ? static_cast<int32_t>((kb + first) % a.page_size)
+                                 : static_cast<int32_t>(sp.begin + kb + first);
+      const int32_t c3 = a.paged ? page : 0;
+      for (int which = 0; which < 2; ++which) {
+        if (!mbar_wait(&kv_empty[slot], phase ^ 1u, abort)) {
+          tc_fail(p.err, abort, kDevErrTmaWait);
+          ok = false;
+          break;
+        }
+        uint8_t* dst = slots + slot * Sh::kTileBytes;
+        const bool mend = which == 1 && ((lo_k | hi_k) & 15) != 0;
+        uint64_t* bar = mend ? &landed : &kv_full[slot];
+        if (lane == 0) mbar_arrive_expect_tx(bar, bytes);
+        __syncwarp();
+        if (load)
+          for (int h = 0; h < Sh::kHalves; ++h)
+            tma_load_4d(dst + h * 16384 + first * 128, which ? &map_v : &map_k, bar, h * 128, head,
+                        c2, c3);
+        __syncwarp();
+        if (mend) {
+          if (!mbar_wait(&landed, static_cast<uint32_t>(landings & 1), abort)) {
+            tc_fail(p.err, abort, kDevErrTmaWait);
+            ok = false;
+          }
+          ++landings;
+          const int a0 = lo_k & ~15, a1 = (hi_k + 15) & ~15;
+          const int dead = (lo_k - a0) + (a1 - hi_k);
+          for (int u = lane; u < dead * 8 * Sh::kHalves; u += 32) {
+            const int i = u / (8 * Sh::kHalves), c = u % (8 * Sh::kHalves);
+            const int r = i < lo_k - a0 ? a0 + i : hi_k + (i - (lo_k - a0));
+            *reinterpret_cast<uint4*>(dst + (c / 8) * 16384 + r * 128 + (c % 8) * 16) =
+                make_uint4(0, 0, 0, 0);
+          }
+          fence_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&kv_full[slot]);
+        }
+        ++issued;
+        if (++slot == Sh::kSlots) {
+          slot = 0;
+          phase ^= 1u;
+        }
+      }
+      page = next_page;
+    }
+    if (*abort) {  // the copies in flight land before the CTA leaves
+      if (n > 0) mbar_wait(&q_full, 0, nullptr);
+      for (int i = issued > Sh::kSlots ? issued - Sh::kSlots : 0; i < issued; ++i)
+        mbar_wait(&kv_full[i % Sh::kSlots], static_cast<uint32_t>((i / Sh::kSlots) & 1), nullptr);
+    }
+  } else if (warp == 9) {
+    // --------------------------------------------------------------- MMAs
+    if (lane == 0 && n > 0) {
+      constexpr int kFmt = std::is_same<T, __half>::value ? 0 : 1;
+      const int k_steps = (a.dim + 15) / 16;
+      const uint32_t id_qk = make_idesc_f16(128, kKeys, kFmt, 0);
+      const uint32_t id_pv = make_idesc_f16(128, k_steps * 16, kFmt, 1);
+      const uint32_t q_addr = smem_u32(sq), kv_addr = smem_u32(slots);
+      auto full = [&](int i, unsigned code) {
+        const bool got = mbar_wait_poll(&kv_full[i % Sh::kSlots],
+                                        static_cast<uint32_t>((i / Sh::kSlots) & 1), abort);
+        if (!got) tc_fail(p.err, abort, code);
+        return got;
+      };
+      auto qk = [&](int t, int i) {  // key tile i of this CTA is ring entry 2 i
+        const uint32_t b = kv_addr + ((2 * i) % Sh::kSlots) * Sh::kTileBytes;
+        const uint32_t q = q_addr + t * Sh::kTileBytes;
+        for (int k = 0; k < k_steps; ++k) {
+          const uint32_t off = (k / 4) * 16384 + (k % 4) * 32;
+          umma_f16(tmem + Sh::kS + t * 128, make_sdesc(q + off, 16, 1024, 2),
+                   make_sdesc(b + off, 16, 1024, 2), id_qk, k > 0);
+        }
+        umma_commit(&s_full[t]);
+      };
+      auto pv = [&](int t, int i) {
+        const uint32_t b = kv_addr + ((2 * i + 1) % Sh::kSlots) * Sh::kTileBytes;
+        const int k0 = v_lo(j0 + i) / 16, k1 = (v_hi(j0 + i) + 15) / 16;
+        for (int k = k0; k < k1; ++k)
+          umma_f16_ta(tmem + Sh::kO + t * DP, tmem + Sh::kS + t * 128 + k * 8,
+                      make_sdesc(b + k * 2048, 16384, 1024, 2), id_pv, i > 0 || k > k0);
+        umma_commit(&o_done[t]);
+      };
+      bool ok = mbar_wait_poll(&q_full, 0, abort);
+      if (!ok) tc_fail(p.err, abort, kDevErrMmaWait);
+      ok = ok && full(0, kDevErrMmaWait);
+      if (ok) {
+        tc_fence_after();
+        if (n0 > 0) qk(0, 0);
+        if (n1 > 0) qk(1, 0);
+        umma_commit(&kv_empty[0]);
+      }
+      for (int i = 0; i < n && ok; ++i) {
+        for (int t = 0; t < 2 && ok; ++t) {
+          const int nt = t == 0 ? n0 : n1;
+          if (i >= nt) continue;
+          ok = mbar_wait_poll(&p_full[t], static_cast<uint32_t>(i & 1), abort);
+          if (!ok) tc_fail(p.err, abort, kDevErrMmaWait);
+          if (!ok || !(ok = full(2 * i + 1, kDevErrMmaWait))) break;
+          tc_fence_after();
+          pv(t, i);
+          if (i + 1 >= nt) continue;
+          if (!(ok = full(2 * i + 2, kDevErrMmaWait))) break;
+          // P is read before the next S is written over it.
+          ok = mbar_wait_poll(&o_done[t], static_cast<uint32_t>(i & 1), abort);
+          if (!ok) {
+            tc_fail(p.err, abort, kDevErrMmaWait);
+            break;
+          }
+          tc_fence_after();
+          qk(t, i + 1);
+        }
+        if (!ok) break;
+        umma_commit(&kv_empty[(2 * i + 1) % Sh::kSlots]);
+        if (i + 1 < n) umma_commit(&kv_empty[(2 * i + 2) % Sh::kSlots]);
+      }
+      // Every MMA completes before tensor memory is freed.
+      umma_commit(&drain);
+      mbar_wait(&drain, 0, nullptr);
+    }
+    __syncwarp();
+  }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
+    // ------------------------------------------------------------ softmax
+    const int t = warp / 4;
+    const int nt = t == 0 ? n0 : n1;
+    const int row = tid % 128;
+    const int tok = row / p.group;
+    const bool real = tok < tokens[t];
+    const int64_t tok_t = t * p.tile_tokens;  // first token of the tile in the pair
+    const int64_t place = place0 + tok_t + tok;
+    const uint32_t lanes = static_cast<uint32_t>((warp % 4) * 32) << 16;
+    const uint32_t ts = tmem + Sh::kS + t * 128 + lanes, to = tmem + Sh::kO + t * DP + lanes;
+    float m = -INFINITY, l = 0.0f;
+    bool ok = true;
+    for (int i = 0; i < nt && ok; ++i) {
+      const int64_t kb = start + static_cast<int64_t>(j0 + i) * kKeys;
+      ok = mbar_wait(&s_full[t], static_cast<uint32_t>(i & 1), abort);
+      if (!ok) {
+        tc_fail(p.err, abort, kDevErrEpiWait);
+        break;
+      }
+      __syncwarp();
+      tc_fence_after();
+      uint32_t s[4][32];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) tmem_ld32_nowait(ts + c * 32, s[c]);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) tmem_wait_ld32(s[c]);
+      const int64_t first_place = place0 + tok_t, last_place = first_place + tokens[t] - 1;
+      if (kb + kKeys > sp.keys || (a.causal && kb + kKeys - 1 > first_place) ||
+          (a.window > 0 && kb <= last_place - a.window)) {
+        int64_t e = sp.keys, b = 0;
+        if (a.causal && place + 1 < e) e = place + 1;
+        if (a.window > 0) b = place - a.window + 1;
+        const int end = static_cast<int>(e - kb < 0 ? 0 : (e - kb > kKeys ? kKeys : e - kb));
+        const int beg = static_cast<int>(b - kb < 0 ? 0 : (b - kb > kKeys ? kKeys : b - kb));
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+          for (int x = 0; x < 32; ++x)
+            if (c * 32 + x >= end || c * 32 + x < beg) s[c][x] = 0xFF800000u;  // -inf
+      }
+      float top[4];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        top[c] = __uint_as_float(s[c][0]);
+#pragma unroll
+        for (int x = 1; x < 32; ++x) top[c] = fmaxf(top[c], __uint_as_float(s[c][x]));
+      }
+      const float m2 = fmaxf(m, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])));
+      const bool grow = (m2 - m) * p.scale_log2 > kGrowLog2;
+      if (__any_sync(~0u, grow)) {
+        const float f = grow ? tc_ex2((m - m2) * p.scale_log2) : 1.0f;
+        if (grow) m = m2;
+        l *= f;
+        if (i > 0) {
+#pragma unroll 1
+          for (int c = 0; c < DP / 32; ++c) {
+            uint32_t o[32];
+            tmem_ld32(to + c * 32, o);
+#pragma unroll
+            for (int x = 0; x < 32; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * f);
+            tmem_st32(to + c * 32, o);
+          }
+        }
+      }
+      const float base = m == -INFINITY ? 0.0f : m * p.scale_log2;
+      float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        uint32_t w[32];
+#pragma unroll
+        for (int x = 0; x < 32; ++x) {
+          const int c = 2 * h + x / 16, y = 2 * (x % 16);
+          const float e0 = tc_ex2(fmaf(__uint_as_float(s[c][y]), p.scale_log2, -base));
+          const float e1 = tc_ex2(fmaf(__uint_as_float(s[c][y + 1]), p.scale_log2, -base));
+          sum[x & 1] += e0;
+          sum[2 + (x & 1)] += e1;
+          w[x] = pack2<T>(e0, e1);
+        }
+        tmem_st32(ts + h * 32, w);
+      }
+      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&p_full[t]);
+    }
+    if (nt > 0 && ok) {
+      ok = mbar_wait(&o_done[t], static_cast<uint32_t>((nt - 1) & 1), abort);
+      if (!ok) tc_fail(p.err, abort, kDevErrEpiWait);
+      __syncwarp();
+      tc_fence_after();
+    }
+    ok = __all_sync(~0u, ok);
+    const int64_t out_row = sp.begin + tok0 + tok_t + tok;
+    const int h = head * p.group + (row - tok * p.group);
+    const int64_t cta = static_cast<int64_t>(blockIdx.x);
+    if (ok) {
+      const float f = p.splits > 1 ? 1.0f : (l == 0.0f ? 0.0f : 1.0f / l);
+      const int64_t at = out_row * a.o_token + h * a.o_head;
+#pragma unroll 1
+      for (int c = 0; c < DP / 32; ++c) {
+        uint32_t o[32];
+        if (nt > 0) {
+          tmem_ld32(to + c * 32, o);
+        } else {
+#pragma unroll
+          for (int x = 0; x < 32; ++x) o[x] = 0;
+        }
+        float v[32];
+#pragma unroll
+        for (int x = 0; x < 32; ++x) v[x] = __uint_as_float(o[x]) * f;
+        if (real) {
+          if (p.splits == 1) {
+#pragma unroll
+            for (int x = 0; x < 32; x += 8)
+              if (c * 32 + x < a.dim) store8<T>(a, at + c * 32 + x, v + x);
+          } else {
+            float4* dst = reinterpret_cast<float4*>(p.part_o + (cta * 256 + t * 128 + row) * DP +
+                                                    c * 32);
+#pragma unroll
+            for (int x = 0; x < 8; ++x)
+              dst[x] = make_float4(v[4 * x], v[4 * x + 1], v[4 * x + 2], v[4 * x + 3]);
+          }
+        }
+      }
+      const float ml = m == -INFINITY ? -INFINITY : m * p.scale_log2;
+      if (real && p.splits > 1) p.part_ml[cta * 256 + t * 128 + row] = make_float2(ml, l);
+      if (real && p.splits == 1 && a.lse != nullptr)
+        a.lse[out_row * a.q_heads + h] =
+            l == 0.0f ? -INFINITY : (log2f(l) + ml) * 0.69314718055994531f;
+    }
+    if (p.splits > 1) {
+      __threadfence();
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+      if (tid == 0) {
+        const unsigned arrived = atomicAdd(p.arrived + seg, 1u);
+        s_last = arrived + 1 == static_cast<unsigned>(p.splits);
+        if (s_last) p.arrived[seg] = 0;
+      }
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+      if (s_last) {
+        __threadfence();
+        // A thread joins 4 columns of a row, all threads side by side.
+        const int64_t c0 = cta - part;
+        for (int u = tid; u < 256 * (DP / 4); u += 256) {
+          const int r = u / (DP / 4), e = (u % (DP / 4)) * 4;
+          const int tt = r / 128, rr = r % 128;
+          const int tk = rr / p.group;
+          if (tk >= tokens[tt]) continue;
+          float mm = -INFINITY;
+          for (int x = 0; x < p.splits; ++x)
+            mm = fmaxf(mm, __ldcg(&p.part_ml[(c0 + x) * 256 + r].x));
+          const float bs = mm == -INFINITY ? 0.0f : mm;
+          float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+          float sum = 0.0f;
+          for (int x = 0; x < p.splits; ++x) {
+            const float2 ml = __ldcg(p.part_ml + (c0 + x) * 256 + r);
+            if (ml.y == 0.0f) continue;  // no key of this part counts
+            const float f = tc_ex2(ml.x - bs);
+            const float4 v =
+                __ldcg(reinterpret_cast<const float4*>(p.part_o + ((c0 + x) * 256 + r) * DP + e));
+            sum = fmaf(ml.y, f, sum);
+            acc.x = fmaf(v.x, f, acc.x);
+            acc.y = fmaf(v.y, f, acc.y);
+            acc.z = fmaf(v.z, f, acc.z);
+            acc.w = fmaf(v.w, f, acc.w);
+          }
+          const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+          const int64_t orow = sp.begin + tok0 + tt * p.tile_tokens + tk;
+          const int oh = head * p.group + (rr - tk * p.group);
+          if (e < a.dim) {
+            const int64_t at = orow * a.o_token + oh * a.o_head + e;
+            const float v[4] = {acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv};
+            if (a.out_dtype == PSPML_DTYPE_S8) {
+              char4 c;
+              c.x = quantise_s8(v[0], a.out_inv_scale, a.out_zero);
+              c.y = quantise_s8(v[1], a.out_inv_scale, a.out_zero);
+              c.z = quantise_s8(v[2], a.out_inv_scale, a.out_zero);
+              c.w = quantise_s8(v[3], a.out_inv_scale, a.out_zero);
+              *reinterpret_cast<char4*>(static_cast<int8_t*>(a.out) + at) = c;
+            } else {
+              *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + at) =
+                  make_uint2(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]));
+            }
+          }
+          if (e == 0 && a.lse != nullptr)
+            a.lse[orow * a.q_heads + oh] =
+                sum == 0.0f ? -INFINITY : (log2f(sum) + bs) * 0.69314718055994531f;
+        }
+      }
+    }
+    tc_fence_before();
+  }
+  __syncthreads();
+  if (warp == 8) {
+    tc_fence_after();
+    tmem_dealloc(tmem, Sh::kCols);
+  }
+}
+
+template <typename T, int DP>
+cudaError_t tc_launch(const TcArgs& p, const CUtensorMap& mq, const CUtensorMap& mk,
+                      const CUtensorMap& mv, unsigned grid, cudaStream_t s) {
+  using Sh = TcShape<DP>;
+  static std::atomic<uint64_t> attr_done{0};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  const uint64_t bit = 1ull << (dev & 63);
+  if ((attr_done.load() & bit) == 0) {
+    const cudaError_t e = cudaFuncSetAttribute(
+        k_attn_tc<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::kSmem);
+    if (e != cudaSuccess) return e;
+    attr_done.fetch_or(bit);
+  }
+  k_attn_tc<T, DP><<<grid, kTcThreads, Sh::kSmem, s>>>(mq, mk, mv, p);
+  return cudaGetLastError();
+}
+
+bool map4(CUtensorMap* m, const void* base, const uint64_t (&dims)[4], const int64_t (&strides)[3],
+          const uint32_t (&box)[4]) {
+  uint64_t d[4], st[3];
+  const uint32_t one[4] = {1, 1, 1, 1};
+  for (int i = 0; i < 4; ++i) d[i] = dims[i];
+  d[0] *= 2;  // bytes
+  // The stride of a dimension of one is never used; any valid one will do.
+  for (int i = 0; i < 3; ++i)
+    st[i] = dims[i + 1] == 1 ? (dims[0] * 2 + 15) / 16 * 16 : static_cast<uint64_t>(strides[i]) * 2;
+  return encode_tensor_map(m, base, 4, d, st, box, one, CU_TENSOR_MAP_SWIZZLE_128B) == CUDA_SUCCESS;
+}
+
+int pow2_gcd128(int x) {
+  int g = 128;
+  while (x % g) g /= 2;
+  return g;
+}
+
+}  // namespace
+
+// What the tensor maps and tiles cover beyond the vector form: a group of at
+// most 128 heads, a positive scale (the running maximum is taken over
+// unscaled products), pages of whole 8-row swizzle groups and strides that
+// are not 0 (a broadcast view).
+bool attn_tc_covers(const AttnArgs& a) {
+  if (a.q_heads / a.kv_heads > 128 || !(a.scale > 0.0f)) return false;
+  if (a.paged && (a.page_size % 8 != 0 || a.n_pages == 0)) return false;
+  if ((a.tokens > 1 && a.q_token == 0) || (a.q_heads > 1 && a.q_head == 0)) return false;
+  if (a.kv_heads > 1 && (a.kv_head == 0 || a.v_head == 0)) return false;
+  if (a.paged) {
+    if ((a.page_size > 1 && a.kv_token == 0) || (a.n_pages > 1 && a.page_stride == 0)) return false;
+  } else if (a.tokens > 1 && (a.kv_token == 0 || a.v_token == 0)) {
+    return false;
+  }
+  return true;
+}
+
+cudaError_t launch_attn_tc(const AttnArgs& a, const AttnWork& w, cudaStream_t s) {
+  const int dp = a.dim <= 64 ? 64 : 128;
+  TcArgs p{};
+  p.a = a;
+  p.err = w.err;
+  p.arrived = w.counters;
+  p.scale_log2 = a.scale * 1.4426950408889634f;
+  p.group = a.q_heads / a.kv_heads;
+  p.tile_tokens = 128 / p.group;
+  p.box_keys = a.paged ? pow2_gcd128(a.page_size) : kKeys;
+
+  // Pairs at most: every sequence may end in a part of one.
+  const int64_t pair_tokens = 2 * p.tile_tokens;
+  int64_t pairs = a.tokens / pair_tokens + a.sequences;
+  if (a.paged)
+    pairs = std::min(pairs, a.sequences * ((a.max_new + pair_tokens - 1) / pair_tokens));
+  const int64_t segments = pairs * a.kv_heads;
+  // Few segments: cut each one's keys so that the parts cover the SMs, with
+  // at least 4 key tiles a part if the sequence is as long as it may be.
+  const int64_t most_keys = a.paged ? a.pages_stride * a.page_size : a.tokens;
+  const int64_t slot = 256 * (dp * static_cast<int64_t>(sizeof(float)) + sizeof(float2));
+  int64_t splits = std::min(w.num_sms / std::max<int64_t>(1, segments), most_keys / (4 * kKeys));
+  splits = std::min(splits, static_cast<int64_t>(w.bytes) / std::max<int64_t>(1, segments * slot));
+  if (segments > kAttnCounters || splits < 1) splits = 1;
+  p.splits = static_cast<int32_t>(splits);
+  const int64_t grid = segments * splits;
+  if (grid > 0x7FFFFFFF) return cudaErrorInvalidValue;
+  p.part_o = reinterpret_cast<float*>(w.base);
+  p.part_ml = reinterpret_cast<float2*>(w.base + grid * 256 * dp * sizeof(float));
+
+  CUtensorMap mq, mk, mv;
+  const uint64_t dim = a.dim, hkv = a.kv_heads, tok = a.tokens;
+  const uint64_t g = p.group;
+  bool ok = map4(&mq, a.q, {dim, g, hkv, tok}, {a.q_head, a.q_head * p.group, a.q_token},
+                 {128, static_cast<uint32_t>(p.group), 1, static_cast<uint32_t>(p.tile_tokens)});
+  const uint32_t box[4] = {128, 1, static_cast<uint32_t>(p.box_keys), 1};
+  if (a.paged) {
+    const uint64_t dims[4] = {dim, hkv, static_cast<uint64_t>(a.page_size),
+                              static_cast<uint64_t>(a.n_pages)};
+    ok = ok && map4(&mk, a.k, dims, {a.kv_head, a.kv_token, a.page_stride}, box) &&
+         map4(&mv, a.v, dims, {a.v_head, a.v_token, a.page_stride}, box);
+  } else {
+    ok = ok && map4(&mk, a.k, {dim, hkv, tok, 1}, {a.kv_head, a.kv_token, 0}, box) &&
+         map4(&mv, a.v, {dim, hkv, tok, 1}, {a.v_head, a.v_token, 0}, box);
+  }
+  if (!ok) return cudaErrorInvalidValue;
+  const unsigned n = static_cast<unsigned>(grid);
+  if (a.dtype == PSPML_DTYPE_F16)
+    return dp == 64 ? tc_launch<__half, 64>(p, mq, mk, mv, n, s)
+                    : tc_launch<__half, 128>(p, mq, mk, mv, n, s);
+  return dp == 64 ? tc_launch<__nv_bfloat16, 64>(p, mq, mk, mv, n, s)
+                  : tc_launch<__nv_bfloat16, 128>(p, mq, mk, mv, n, s);
+}
+
+}  // namespace pspml
