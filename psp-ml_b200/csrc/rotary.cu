@@ -11,6 +11,8 @@
 // to the output type.
 #include <cuda_runtime.h>
 
+#include <algorithm>
+
 #include "attention.h"
 
 namespace pspml {
@@ -85,9 +87,191 @@ __global__ void __launch_bounds__(kThreads) k_rotary_any(const RotaryArgs a, con
   out[ey] = from_f32<Out>(x * sn + y * cs);
 }
 
+// V neighbouring elements, moved in pieces of at most 16 bytes.
+template <int Bytes> struct Piece;
+template <> struct Piece<4> { using type = uint32_t; };
+template <> struct Piece<8> { using type = uint2; };
+template <> struct Piece<16> { using type = uint4; };
+template <typename E, int V>
+struct Elems {
+  static constexpr int kPiece = V * sizeof(E) < 16 ? V * sizeof(E) : 16;
+  static constexpr int kPieces = V * sizeof(E) / kPiece;
+  using P = typename Piece<kPiece>::type;
+  P p[kPieces];
+  __device__ __forceinline__ void load(const E* s) {
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) p[i] = reinterpret_cast<const P*>(s)[i];
+  }
+  __device__ __forceinline__ void store(E* d) const {
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) reinterpret_cast<P*>(d)[i] = p[i];
+  }
+  __device__ __forceinline__ uint32_t& word(int i) { return reinterpret_cast<uint32_t*>(p)[i]; }
+  // Values as floats; `bias` is 2^23 + 128 + zero point for S8.
+  __device__ __forceinline__ void values(float* v, float scale, float bias) {
+    if constexpr (sizeof(E) == 1) {
+      // A byte with its sign bit flipped is q + 128; as the low byte of the
+      // float 2^23 it adds to it exactly, with no conversion instruction.
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+        v[i] = scale * (__uint_as_float(__byte_perm(word(i / 4) ^ 0x80808080u, 0x4B000000u,
+                                                    0x7540 + (i % 4))) - bias);
+    } else {
+#pragma unroll
+      for (int i = 0; i < V; ++i) v[i] = to_f32(reinterpret_cast<const E*>(p)[i]);
+    }
+  }
+  __device__ __forceinline__ void round(const float* v) {
+    if constexpr (sizeof(E) == 4) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) word(i) = __float_as_uint(v[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < V / 2; ++i) word(i) = pack2<E>(v[2 * i], v[2 * i + 1]);
+    }
+  }
+};
+
+// Vector form.  The bytes bound it, so a thread moves whole vectors: it
+// takes V pairs of one token (elements j*V.. of both halves, or 2V
+// neighbours) or V passed-through elements, finds their sines and cosines
+// once, and walks every `lanes`-th head with kBatch heads' loads in flight.
+// Neighbouring threads take neighbouring units, then neighbouring heads, so
+// a step of a warp covers whole heads side by side in memory.
+constexpr int kBatch = 4;
+template <typename In, typename Out, int V, bool kHalf>
+__global__ void __launch_bounds__(kThreads)
+    k_rotary_vec(const RotaryArgs a, const int units, const int lanes) {
+  const int64_t idx = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
+  const int64_t t = idx / (units * lanes);
+  if (t >= a.tokens) return;
+  const int rest = static_cast<int>(idx - t * (units * lanes));
+  const int hl = rest / units, u = rest - hl * units;
+  const int turned = a.rot / (2 * V);      // units that hold pairs
+  const bool pairs = u < turned;
+  const int ex = pairs ? (kHalf ? u * V : u * 2 * V) : a.rot + (u - turned) * V;
+  const int ey = kHalf ? ex + a.rot / 2 : ex + V;
+  const int heads = a.q.heads + a.k.heads + a.v.heads;
+  const float bias = 8388736.0f + static_cast<float>(a.zero);
+
+  int64_t cached = 0;                       // offset of the token's slot
+  bool keep = true;
+  if (a.slots != nullptr) {
+    const int64_t slot = a.slots[t];
+    keep = slot >= 0 && slot < a.slots_total;
+    if (keep) {
+      const int64_t page = (slot >> 32) == 0 ? static_cast<uint32_t>(slot) /
+                                                   static_cast<uint32_t>(a.page_size)
+                                             : slot / a.page_size;
+      cached = page * a.page_stride + (slot - page * a.page_size) * a.slot_stride;
+    }
+  }
+  float sn[V], cs[V];
+  if (pairs) {
+    const unsigned long long at =
+        static_cast<unsigned long long>(static_cast<long long>(a.positions[t]));
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const long long turns = static_cast<long long>(at * a.freq[u * V + i]);
+      sincospif(static_cast<float>(turns) * 0x1p-63f, &sn[i], &cs[i]);
+      sn[i] *= a.amplitude;
+      cs[i] *= a.amplitude;
+    }
+  }
+
+  for (int hb = hl; hb < heads; hb += kBatch * lanes) {
+    Elems<In, V> x[kBatch], y[kBatch];
+    Out* dst[kBatch];
+    bool turn[kBatch];
+#pragma unroll
+    for (int b = 0; b < kBatch; ++b) {
+      int h = hb + b * lanes;
+      dst[b] = nullptr;
+      if (h >= heads) continue;
+      const bool is_q = h < a.q.heads;
+      if (!is_q) h -= a.q.heads;
+      const bool is_k = !is_q && h < a.k.heads;
+      if (!is_q && !is_k) h -= a.k.heads;
+      turn[b] = is_q || is_k;
+      const RotaryView& w = is_q ? a.q : (is_k ? a.k : a.v);
+      const bool to_cache = !is_q && a.slots != nullptr;
+      if (to_cache && !keep) continue;
+      dst[b] = static_cast<Out*>(w.out) + (to_cache ? cached : t * w.out_token) + h * w.out_head;
+      const In* src = static_cast<const In*>(w.in) + t * w.in_token + h * w.in_head;
+      x[b].load(src + ex);
+      if (pairs) y[b].load(src + ey);
+    }
+#pragma unroll
+    for (int b = 0; b < kBatch; ++b) {
+      if (dst[b] == nullptr) continue;
+      float v[2 * V];
+      x[b].values(v, a.scale, bias);
+      if (pairs) y[b].values(v + V, a.scale, bias);
+      if (pairs && turn[b]) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          float& p = kHalf ? v[i] : v[2 * i];
+          float& q = kHalf ? v[V + i] : v[2 * i + 1];
+          const float s = p * cs[i] - q * sn[i];
+          q = p * sn[i] + q * cs[i];
+          p = s;
+        }
+      }
+      Elems<Out, V> o;
+      o.round(v);
+      o.store(dst[b] + ex);
+      if (pairs) {
+        o.round(v + V);
+        o.store(dst[b] + ey);
+      }
+    }
+  }
+}
+
+// Whether every vector of V elements is aligned in memory.
+template <typename In, typename Out, int V>
+bool vectors_fit(const RotaryArgs& a) {
+  if (a.rot % (2 * V) != 0 || a.dim % V != 0) return false;
+  const auto fits = [](const void* p, int64_t bits, int bytes) {
+    const int n = bytes < 16 ? bytes : 16;
+    return reinterpret_cast<uintptr_t>(p) % n == 0 && (bits * (bytes / V)) % n == 0;
+  };
+  const int in = V * sizeof(In), out = V * sizeof(Out);
+  for (const RotaryView* w : {&a.q, &a.k, &a.v}) {
+    if (w->heads == 0) continue;
+    if (!fits(w->in, w->in_token | w->in_head, in) || !fits(w->out, w->out_token | w->out_head, out))
+      return false;
+  }
+  return a.slots == nullptr || fits(nullptr, a.page_stride | a.slot_stride, out);
+}
+
+template <typename In, typename Out, int V>
+cudaError_t launch_vec(const RotaryArgs& a, int num_sms, cudaStream_t s) {
+  const int heads = a.q.heads + a.k.heads + a.v.heads;
+  const int units = a.dim / V - a.rot / (2 * V);
+  // Threads a token and unit: four when tokens are many, so that a thread
+  // uses its angles for a quarter of the heads; more until the machine is
+  // full of threads, up to one a head.
+  int lanes = std::min(4, heads);
+  while (lanes < heads && a.tokens * units * lanes < static_cast<int64_t>(num_sms) * 1024)
+    lanes = std::min(2 * lanes, heads);
+  const int64_t blocks = (a.tokens * units * lanes + kThreads - 1) / kThreads;
+  if (blocks > 0x7FFFFFFF) return cudaErrorInvalidValue;
+  const unsigned grid = static_cast<unsigned>(blocks);
+  if (a.layout == PSPML_ROTARY_HALF)
+    k_rotary_vec<In, Out, V, true><<<grid, kThreads, 0, s>>>(a, units, lanes);
+  else
+    k_rotary_vec<In, Out, V, false><<<grid, kThreads, 0, s>>>(a, units, lanes);
+  return cudaGetLastError();
+}
+
 template <typename In, typename Out>
 cudaError_t launch_io(const RotaryArgs& a, int num_sms, cudaStream_t s) {
-  (void)num_sms;
+  // Eight elements where 16-byte vectors of them fit, four where half-size
+  // ones do (a rotated part that is no multiple of 16).
+  if constexpr (sizeof(In) <= 2 && sizeof(Out) <= 2)
+    if (vectors_fit<In, Out, 8>(a)) return launch_vec<In, Out, 8>(a, num_sms, s);
+  if (vectors_fit<In, Out, 4>(a)) return launch_vec<In, Out, 4>(a, num_sms, s);
   const int heads = a.q.heads + a.k.heads + a.v.heads;
   const int units = a.dim - a.rot / 2;
   const int64_t total = a.tokens * heads * units;

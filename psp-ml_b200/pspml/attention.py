@@ -12,12 +12,14 @@ from __future__ import annotations
 
 import ctypes
 import math
+import struct
 
 import numpy as np
 import torch
 
 from . import capi
 
+_ref = ctypes.byref
 _DTYPES = {torch.float32: capi.DTYPE_F32, torch.float16: capi.DTYPE_F16,
            torch.bfloat16: capi.DTYPE_BF16}
 _LAYOUTS = {"half": capi.ROTARY_HALF, "interleaved": capi.ROTARY_INTERLEAVED}
@@ -35,32 +37,36 @@ class Quantised:
 
 
 def _on(device: int, t: torch.Tensor, what: str) -> None:
-    if t.device.index != device or t.device.type != "cuda":
+    if t.get_device() != device:
         raise ValueError(f"{what} is on {t.device}, the context on cuda:{device}")
 
 
-def heads(x, device: int, what: str = "tensor") -> capi.Heads:
-    """The C view of a [tokens][heads][dim] tensor (or a Quantised one)."""
-    scale, zero = 1.0, 0
-    if isinstance(x, Quantised):
-        x, scale, zero = x.tensor, x.scale, x.zero_point
-        dtype = capi.DTYPE_S8
+# struct pspml_heads as bytes: half the cost of filling a ctypes.Structure.
+_pack_heads = struct.Struct("@Pqqiiiifi").pack
+
+
+def heads(x, device: int, what: str = "tensor") -> bytes:
+    """The C view (struct pspml_heads) of a [tokens][heads][dim] tensor or a Quantised one."""
+    if type(x) is Quantised:
+        x, scale, zero, dtype = x.tensor, x.scale, x.zero_point, capi.DTYPE_S8
     else:
-        dtype = _DTYPES.get(x.dtype)
+        scale, zero, dtype = 1.0, 0, _DTYPES.get(x.dtype)
         if dtype is None:
             raise ValueError(f"{what}: dtype {x.dtype} is not float32, float16 or bfloat16")
-    _on(device, x, what)
-    n, h, d = x.shape
+    if x.get_device() != device:
+        _on(device, x, what)
+    _, h, d = x.shape
     st, sh, sd = x.stride()
     if sd != 1 and d != 1:
         raise ValueError(f"{what}: a head's elements are not contiguous")
-    return capi.Heads(x.data_ptr(), st, sh, h, d, dtype, zero, scale, 0)
+    return _pack_heads(x.data_ptr(), st, sh, h, d, dtype, zero, scale, 0)
 
 
 def _index(x: torch.Tensor, dtype, n: int, device: int, what: str) -> int:
-    if x.dtype != dtype or not x.is_contiguous() or x.numel() != n:
+    if x.dtype is not dtype or x.numel() != n or not x.is_contiguous():
         raise ValueError(f"{what}: needs {n} contiguous {dtype}")
-    _on(device, x, what)
+    if x.get_device() != device:
+        _on(device, x, what)
     return x.data_ptr()
 
 
@@ -78,8 +84,8 @@ class Rotary:
         self.desc = rotary_desc(head_dim, rot_dim, layout, base, scaling, factor, original_len,
                                 low, high, amplitude)
         self.handle = ctypes.c_void_p()
-        capi.call("pspml_rotary_create", ctx.handle, ctypes.byref(self.desc),
-                  ctypes.byref(self.handle))
+        capi.call("pspml_rotary_create", ctx.handle, _ref(self.desc),
+                  _ref(self.handle))
 
     def close(self) -> None:
         if self.handle:
@@ -102,7 +108,7 @@ def rotary_desc(head_dim, rot_dim=None, layout="half", base=10000.0, scaling="no
 def rotary_frequencies(desc: capi.RotaryDesc) -> np.ndarray:
     """Turns per position of each pair, as 64-bit binary fractions of a turn (no device)."""
     out = np.zeros(max(1, desc.rot_dim // 2), np.uint64)
-    capi.call("pspml_rotary_frequencies", ctypes.byref(desc), out.ctypes.data)
+    capi.call("pspml_rotary_frequencies", _ref(desc), out.ctypes.data)
     return out[:desc.rot_dim // 2]
 
 
@@ -141,7 +147,7 @@ def rotary_apply(rotary: Rotary, positions: torch.Tensor, q, q_out, k=None, k_ou
     """q_out, k_out = q, k turned to their int32 positions; outputs may be the inputs."""
     n, dev = _tokens(q), rotary.ctx.device
     _same_tokens(n, q_out, k, k_out)
-    refs = [ctypes.byref(heads(x, dev, w)) if x is not None else None
+    refs = [heads(x, dev, w) if x is not None else None
             for x, w in ((q, "q"), (q_out, "q_out"), (k, "k"), (k_out, "k_out"))]
     capi.call("pspml_rotary_apply", rotary.handle, n,
               _index(positions, torch.int32, n, dev, "positions"), *refs, stream)
@@ -154,11 +160,11 @@ def rotary_append(rotary: Rotary, positions: torch.Tensor, slots: torch.Tensor, 
     n, dev = _tokens(k), rotary.ctx.device
     _same_tokens(n, q, q_out, v)
     _on(dev, cache.k, "cache")
-    refs = [ctypes.byref(heads(x, dev, w)) if x is not None else None
+    refs = [heads(x, dev, w) if x is not None else None
             for x, w in ((q, "q"), (q_out, "q_out"), (k, "k"), (v, "v"))]
     capi.call("pspml_rotary_append", rotary.handle, n,
               _index(positions, torch.int32, n, dev, "positions"),
-              _index(slots, torch.int64, n, dev, "slots"), *refs, ctypes.byref(cache.view), stream)
+              _index(slots, torch.int64, n, dev, "slots"), *refs, _ref(cache.view), stream)
 
 
 def _desc(dim: int, causal: bool, window: int, scale: float | None) -> capi.AttentionDesc:
@@ -179,10 +185,10 @@ def prompt(ctx: capi.Context, q, k, v, starts: torch.Tensor, out, lse=None, caus
     n, dev = q.shape[0], ctx.device
     _same_tokens(n, k, v, out)
     d = _desc(q.shape[2], causal, window, scale)
-    capi.call("pspml_attention_prompt", ctx.handle, ctypes.byref(d), n, starts.numel() - 1,
+    capi.call("pspml_attention_prompt", ctx.handle, _ref(d), n, starts.numel() - 1,
               _index(starts, torch.int32, starts.numel(), dev, "starts"),
-              ctypes.byref(heads(q, dev, "q")), ctypes.byref(heads(k, dev, "k")),
-              ctypes.byref(heads(v, dev, "v")), ctypes.byref(heads(out, dev, "out")),
+              heads(q, dev, "q"), heads(k, dev, "k"),
+              heads(v, dev, "v"), heads(out, dev, "out"),
               _lse(lse, q, dev), stream)
 
 
@@ -201,8 +207,8 @@ def cached(ctx: capi.Context, q, cache: KvCache, starts: torch.Tensor, lengths: 
             not pages.is_contiguous():
         raise ValueError("pages: needs a contiguous int32 row for each sequence")
     d = _desc(q.shape[2], causal, window, scale)
-    capi.call("pspml_attention_cached", ctx.handle, ctypes.byref(d), n, seqs, max_new,
+    capi.call("pspml_attention_cached", ctx.handle, _ref(d), n, seqs, max_new,
               _index(starts, torch.int32, seqs + 1, dev, "starts"),
               _index(lengths, torch.int32, seqs, dev, "lengths"), pages.data_ptr(), pages.shape[1],
-              ctypes.byref(heads(q, dev, "q")), ctypes.byref(cache.view),
-              ctypes.byref(heads(out, dev, "out")), _lse(lse, q, dev), stream)
+              heads(q, dev, "q"), _ref(cache.view),
+              heads(out, dev, "out"), _lse(lse, q, dev), stream)

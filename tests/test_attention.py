@@ -189,3 +189,5 @@ def test_struct_layouts():
     assert ctypes.sizeof(capi.KvCacheView) == 64
     assert ctypes.sizeof(capi.RotaryDesc) == 64
     assert ctypes.sizeof(capi.AttentionDesc) == 16
+    packed = attention._pack_heads(4096, 5, 6, 7, 8, 9, -10, 0.5, 0)
+    assert packed == bytes(capi.Heads(4096, 5, 6, 7, 8, 9, -10, 0.5, 0))
