@@ -12,6 +12,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "attention.h"
 
@@ -132,29 +133,109 @@ struct Elems {
   }
 };
 
-// Vector form.  The bytes bound it, so a thread moves whole vectors: it
-// takes V pairs of one token (elements j*V.. of both halves, or 2V
-// neighbours) or V passed-through elements, finds their sines and cosines
-// once, and walks every `lanes`-th head with kBatch heads' loads in flight.
-// Neighbouring threads take neighbouring units, then neighbouring heads, so
-// a step of a warp covers whole heads side by side in memory.
+// Vector form.  The bytes bound it, so a thread moves whole vectors and
+// little else: it takes V pairs of one token (elements j*V.. of both halves,
+// or 2V neighbours), or V passed-through elements, and walks every
+// `lanes`-th head of q, k and v with kBatch heads' loads in flight.  Blocks
+// of pairs come first, then blocks of passed-through elements, so that no
+// warp runs both.  Neighbouring threads take neighbouring units, then
+// neighbouring heads, then tokens; a block finds the sines and cosines of
+// its tokens once, in shared memory.
 constexpr int kBatch = 4;
-template <typename In, typename Out, int V, bool kHalf>
-__global__ void __launch_bounds__(kThreads)
-    k_rotary_vec(const RotaryArgs a, const int units, const int lanes) {
-  const int64_t idx = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
-  const int64_t t = idx / (units * lanes);
-  if (t >= a.tokens) return;
-  const int rest = static_cast<int>(idx - t * (units * lanes));
-  const int hl = rest / units, u = rest - hl * units;
-  const int turned = a.rot / (2 * V);      // units that hold pairs
-  const bool pairs = u < turned;
-  const int ex = pairs ? (kHalf ? u * V : u * 2 * V) : a.rot + (u - turned) * V;
-  const int ey = kHalf ? ex + a.rot / 2 : ex + V;
-  const int heads = a.q.heads + a.k.heads + a.v.heads;
-  const float bias = 8388736.0f + static_cast<float>(a.zero);
 
-  int64_t cached = 0;                       // offset of the token's slot
+struct RotaryPlan {
+  int32_t lanes;                     // heads side by side in a block
+  int32_t pair_units, pass_units;    // threads a head
+  int32_t pair_tokens, pass_tokens;  // tokens a block
+  int64_t pair_blocks;
+};
+
+// One view's heads hl, hl + step, ... of a token.
+template <typename In, typename Out, int V, bool kHalf, bool kPairs>
+__device__ __forceinline__ void rotary_view(const RotaryArgs& a, const RotaryView& w, int64_t t,
+                                            int64_t out_off, int hl, int step, int ex, int ey,
+                                            bool turn, const float* cs, const float* sn) {
+  const In* in = static_cast<const In*>(w.in) + t * w.in_token + hl * w.in_head;
+  Out* out = static_cast<Out*>(w.out) + out_off + hl * w.out_head;
+  const int64_t in_step = step * w.in_head, out_step = step * w.out_head;
+  const float bias = 8388736.0f + static_cast<float>(a.zero);
+  for (int h = hl; h < w.heads; h += kBatch * step) {
+    Elems<In, V> x[kBatch], y[kBatch];
+#pragma unroll
+    for (int b = 0; b < kBatch; ++b)
+      if (h + b * step < w.heads) {
+        x[b].load(in + b * in_step + ex);
+        if constexpr (kPairs) y[b].load(in + b * in_step + ey);
+      }
+#pragma unroll
+    for (int b = 0; b < kBatch; ++b)
+      if (h + b * step < w.heads) {
+        Elems<Out, V> o;
+        if constexpr (!kPairs && std::is_same<In, Out>::value) {
+          x[b].store(out + b * out_step + ex);
+        } else if constexpr (!kPairs) {
+          float v[V];
+          x[b].values(v, a.scale, bias);
+          o.round(v);
+          o.store(out + b * out_step + ex);
+        } else {
+          float v[2 * V];
+          x[b].values(v, a.scale, bias);
+          y[b].values(v + V, a.scale, bias);
+          if (turn) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+              float& p = kHalf ? v[i] : v[2 * i];
+              float& q = kHalf ? v[V + i] : v[2 * i + 1];
+              const float s = p * cs[i] - q * sn[i];
+              q = p * sn[i] + q * cs[i];
+              p = s;
+            }
+          }
+          o.round(v);
+          o.store(out + b * out_step + ex);
+          o.round(v + V);
+          o.store(out + b * out_step + ey);
+        }
+      }
+    in += kBatch * in_step;
+    out += kBatch * out_step;
+  }
+}
+
+template <typename In, typename Out, int V, bool kHalf>
+__global__ void __launch_bounds__(kThreads, 6)
+    k_rotary_vec(const RotaryArgs a, const RotaryPlan pl) {
+  __shared__ float2 s_turn[kThreads * V];  // [token][pair]: pair_tokens * pair_units <= kThreads
+  const bool pairs = blockIdx.x < pl.pair_blocks;
+  const int units = pairs ? pl.pair_units : pl.pass_units;
+  const int tokens = pairs ? pl.pair_tokens : pl.pass_tokens;
+  const int64_t t0 = (pairs ? static_cast<int64_t>(blockIdx.x)
+                            : static_cast<int64_t>(blockIdx.x) - pl.pair_blocks) * tokens;
+  const int tl = threadIdx.x / (units * pl.lanes);
+  const int rest = threadIdx.x - tl * (units * pl.lanes);
+  const int u = rest % units;
+  const int hl = blockIdx.y * pl.lanes + rest / units, step = gridDim.y * pl.lanes;
+  const int64_t t = t0 + tl;
+  const int half = a.rot / 2;
+
+  if (pairs) {
+    for (int i = threadIdx.x; i < tokens * half; i += kThreads) {
+      const int64_t ti = t0 + i / half;
+      if (ti < a.tokens) {
+        const unsigned long long at =
+            static_cast<unsigned long long>(static_cast<long long>(a.positions[ti]));
+        float sn, cs;
+        sincospif(static_cast<float>(static_cast<long long>(at * a.freq[i % half])) * 0x1p-63f, &sn,
+                  &cs);
+        s_turn[i] = make_float2(cs * a.amplitude, sn * a.amplitude);
+      }
+    }
+    __syncthreads();
+  }
+  if (tl >= tokens || t >= a.tokens) return;
+
+  int64_t cached = 0;  // offset of the token's slot
   bool keep = true;
   if (a.slots != nullptr) {
     const int64_t slot = a.slots[t];
@@ -166,72 +247,37 @@ __global__ void __launch_bounds__(kThreads)
       cached = page * a.page_stride + (slot - page * a.page_size) * a.slot_stride;
     }
   }
-  float sn[V], cs[V];
+  const int64_t k_off = a.slots != nullptr ? cached : t * a.k.out_token;
   if (pairs) {
-    const unsigned long long at =
-        static_cast<unsigned long long>(static_cast<long long>(a.positions[t]));
+    float cs[V], sn[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      const long long turns = static_cast<long long>(at * a.freq[u * V + i]);
-      sincospif(static_cast<float>(turns) * 0x1p-63f, &sn[i], &cs[i]);
-      sn[i] *= a.amplitude;
-      cs[i] *= a.amplitude;
+      const float2 c = s_turn[tl * half + u * V + i];
+      cs[i] = c.x;
+      sn[i] = c.y;
     }
-  }
-
-  for (int hb = hl; hb < heads; hb += kBatch * lanes) {
-    Elems<In, V> x[kBatch], y[kBatch];
-    Out* dst[kBatch];
-    bool turn[kBatch];
-#pragma unroll
-    for (int b = 0; b < kBatch; ++b) {
-      int h = hb + b * lanes;
-      dst[b] = nullptr;
-      if (h >= heads) continue;
-      const bool is_q = h < a.q.heads;
-      if (!is_q) h -= a.q.heads;
-      const bool is_k = !is_q && h < a.k.heads;
-      if (!is_q && !is_k) h -= a.k.heads;
-      turn[b] = is_q || is_k;
-      const RotaryView& w = is_q ? a.q : (is_k ? a.k : a.v);
-      const bool to_cache = !is_q && a.slots != nullptr;
-      if (to_cache && !keep) continue;
-      dst[b] = static_cast<Out*>(w.out) + (to_cache ? cached : t * w.out_token) + h * w.out_head;
-      const In* src = static_cast<const In*>(w.in) + t * w.in_token + h * w.in_head;
-      x[b].load(src + ex);
-      if (pairs) y[b].load(src + ey);
-    }
-#pragma unroll
-    for (int b = 0; b < kBatch; ++b) {
-      if (dst[b] == nullptr) continue;
-      float v[2 * V];
-      x[b].values(v, a.scale, bias);
-      if (pairs) y[b].values(v + V, a.scale, bias);
-      if (pairs && turn[b]) {
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-          float& p = kHalf ? v[i] : v[2 * i];
-          float& q = kHalf ? v[V + i] : v[2 * i + 1];
-          const float s = p * cs[i] - q * sn[i];
-          q = p * sn[i] + q * cs[i];
-          p = s;
-        }
-      }
-      Elems<Out, V> o;
-      o.round(v);
-      o.store(dst[b] + ex);
-      if (pairs) {
-        o.round(v + V);
-        o.store(dst[b] + ey);
-      }
-    }
+    const int ex = kHalf ? u * V : u * 2 * V, ey = kHalf ? ex + half : ex + V;
+    rotary_view<In, Out, V, kHalf, true>(a, a.q, t, t * a.q.out_token, hl, step, ex, ey, true, cs,
+                                         sn);
+    if (!keep) return;
+    rotary_view<In, Out, V, kHalf, true>(a, a.k, t, k_off, hl, step, ex, ey, true, cs, sn);
+    rotary_view<In, Out, V, kHalf, true>(a, a.v, t, cached, hl, step, ex, ey, false, cs, sn);
+  } else {
+    const int e = a.rot + u * V;
+    rotary_view<In, Out, V, kHalf, false>(a, a.q, t, t * a.q.out_token, hl, step, e, 0, false,
+                                          nullptr, nullptr);
+    if (!keep) return;
+    rotary_view<In, Out, V, kHalf, false>(a, a.k, t, k_off, hl, step, e, 0, false, nullptr, nullptr);
+    rotary_view<In, Out, V, kHalf, false>(a, a.v, t, cached, hl, step, e, 0, false, nullptr, nullptr);
   }
 }
 
 // Whether every vector of V elements is aligned in memory.
 template <typename In, typename Out, int V>
 bool vectors_fit(const RotaryArgs& a) {
-  if (a.rot % (2 * V) != 0 || a.dim % V != 0) return false;
+  if (a.rot % (2 * V) != 0 || a.dim % V != 0 || a.rot / (2 * V) > kThreads ||
+      (a.dim - a.rot) / V > kThreads)
+    return false;
   const auto fits = [](const void* p, int64_t bits, int bytes) {
     const int n = bytes < 16 ? bytes : 16;
     return reinterpret_cast<uintptr_t>(p) % n == 0 && (bits * (bytes / V)) % n == 0;
@@ -247,21 +293,35 @@ bool vectors_fit(const RotaryArgs& a) {
 
 template <typename In, typename Out, int V>
 cudaError_t launch_vec(const RotaryArgs& a, int num_sms, cudaStream_t s) {
-  const int heads = a.q.heads + a.k.heads + a.v.heads;
-  const int units = a.dim / V - a.rot / (2 * V);
-  // Threads a token and unit: four when tokens are many, so that a thread
-  // uses its angles for a quarter of the heads; more until the machine is
-  // full of threads, up to one a head.
-  int lanes = std::min(4, heads);
-  while (lanes < heads && a.tokens * units * lanes < static_cast<int64_t>(num_sms) * 1024)
-    lanes = std::min(2 * lanes, heads);
-  const int64_t blocks = (a.tokens * units * lanes + kThreads - 1) / kThreads;
+  const int heads = std::max({a.q.heads, a.k.heads, a.v.heads});
+  RotaryPlan pl{};
+  pl.pair_units = a.rot / (2 * V);
+  pl.pass_units = (a.dim - a.rot) / V;
+  const int units = pl.pair_units + pl.pass_units, most = std::max(pl.pair_units, pl.pass_units);
+  // Four heads side by side when tokens are many: long runs in memory, and
+  // a thread uses its angles for a quarter of the heads.  With few tokens
+  // the heads are spread over blocks until the machine is full of threads.
+  pl.lanes = std::max(1, std::min({4, heads, kThreads / most}));
+  int split = 1;
+  while (split * pl.lanes < heads &&
+         a.tokens * units * pl.lanes * split < static_cast<int64_t>(num_sms) * 1024)
+    split *= 2;
+  int64_t blocks = 0;
+  if (pl.pair_units > 0) {
+    pl.pair_tokens = kThreads / (pl.pair_units * pl.lanes);
+    pl.pair_blocks = (a.tokens + pl.pair_tokens - 1) / pl.pair_tokens;
+    blocks += pl.pair_blocks;
+  }
+  if (pl.pass_units > 0) {
+    pl.pass_tokens = kThreads / (pl.pass_units * pl.lanes);
+    blocks += (a.tokens + pl.pass_tokens - 1) / pl.pass_tokens;
+  }
   if (blocks > 0x7FFFFFFF) return cudaErrorInvalidValue;
-  const unsigned grid = static_cast<unsigned>(blocks);
+  const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>(split));
   if (a.layout == PSPML_ROTARY_HALF)
-    k_rotary_vec<In, Out, V, true><<<grid, kThreads, 0, s>>>(a, units, lanes);
+    k_rotary_vec<In, Out, V, true><<<grid, kThreads, 0, s>>>(a, pl);
   else
-    k_rotary_vec<In, Out, V, false><<<grid, kThreads, 0, s>>>(a, units, lanes);
+    k_rotary_vec<In, Out, V, false><<<grid, kThreads, 0, s>>>(a, pl);
   return cudaGetLastError();
 }
 
