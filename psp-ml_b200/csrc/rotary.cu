@@ -141,7 +141,7 @@ struct Elems {
 // warp runs both.  Neighbouring threads take neighbouring units, then
 // neighbouring heads, then tokens; a block finds the sines and cosines of
 // its tokens once, in shared memory.
-constexpr int kBatch = 4;
+constexpr int kBatch = 2;
 
 struct RotaryPlan {
   int32_t lanes;                     // heads side by side in a block
@@ -204,7 +204,7 @@ __device__ __forceinline__ void rotary_view(const RotaryArgs& a, const RotaryVie
 }
 
 template <typename In, typename Out, int V, bool kHalf>
-__global__ void __launch_bounds__(kThreads, 6)
+__global__ void __launch_bounds__(kThreads, 8)
     k_rotary_vec(const RotaryArgs a, const RotaryPlan pl) {
   __shared__ float2 s_turn[kThreads * V];  // [token][pair]: pair_tokens * pair_units <= kThreads
   const bool pairs = blockIdx.x < pl.pair_blocks;
