@@ -15,8 +15,9 @@
 //                   output is rescaled only when the maximum has grown by
 //                   more than 2^8 since the last time, by the same threads
 //   warp 8          TMA loads: Q once, K and V tiles through a ring of slots
-//   warp 9          (10 and 11 idle) one thread issues the MMAs: P V of a tile, then the next
-//                   Q K^T of the same tile once P has been read
+//   warp 9          one thread issues the MMAs: P V of a tile, then the next
+//                   Q K^T of the same tile once P has been read (warps 10
+//                   and 11 only fill the warpgroup)
 // Tensor memory: S/P of A and B (128 columns each), O of A and B.
 //
 // Keys that no row of the CTA sees are not loaded; the values between such a
@@ -46,12 +47,13 @@ CUresult encode_tensor_map(CUtensorMap* map, const void* base, int rank, const u
 namespace {
 
 // Three warpgroups: 168 registers a thread at launch, of which the softmax
-// groups take 208 and the third keeps 88 (128 * (2 * 208 + 88) = 384 * 168).
+// groups take 200 and the third keeps 104 (128 * (2 * 200 + 104) = 384 * 168).
 constexpr int kTcThreads = 384;
-constexpr int kSoftmaxRegs = 208;
-constexpr int kOtherRegs = 88;
+constexpr int kSoftmaxRegs = 200;
+constexpr int kOtherRegs = 104;
 constexpr int kTcWarps = kTcThreads / 32;
 constexpr int kKeys = 128;        // keys a tile
+constexpr int kEmuPairs = 0;      // of 8 pairs of exponentials, those on the FMA pipe
 constexpr float kGrowLog2 = 8.0f; // largest stale maximum, as a power of two
 
 struct TcArgs {
@@ -81,6 +83,61 @@ __device__ __forceinline__ float tc_ex2(float x) {
   return y;
 }
 
+// Two floats in one 64-bit register, and the packed arithmetic on them.
+__device__ __forceinline__ uint64_t f2(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ void f2_get(uint64_t v, float& lo, float& hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+__device__ __forceinline__ uint64_t f2_fma(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t f2_add(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
+// 2^x of two floats in [-inf, 127) on the FMA pipe: x = n + f with n the
+// nearest integer (found by adding 1.5 * 2^23, whose low bits then hold n),
+// 2^f by the polynomial of least relative error on [-1/2, 1/2] (fitted by
+// exchange; 2^-13.7 of degree 3 for BF16 weights, 2^-18.5 of degree 4 for
+// F16, a sixteenth of their rounding or less), n added to the exponent.  x
+// is cut at -126.
+template <typename T>
+__device__ __forceinline__ uint64_t f2_exp2(uint64_t x) {
+  float a, b;
+  f2_get(x, a, b);
+  x = f2(fmaxf(a, -126.0f), fmaxf(b, -126.0f));
+  const uint64_t magic = f2(12582912.0f, 12582912.0f);
+  const uint64_t n = f2_add(x, magic);
+  const uint64_t r = f2_add(n, f2(-12582912.0f, -12582912.0f));
+  const uint64_t f = f2_fma(r, f2(-1.0f, -1.0f), x);
+  uint64_t p;
+  if constexpr (std::is_same<T, __half>::value) {
+    p = f2_fma(f2(0.009570102207362652f, 0.009570102207362652f), f,
+               f2(0.05591785907745361f, 0.05591785907745361f));
+    p = f2_fma(p, f, f2(0.240247443318367f, 0.240247443318367f));
+    p = f2_fma(p, f, f2(0.6931217908859253f, 0.6931217908859253f));
+    p = f2_fma(p, f, f2(0.9999992847442627f, 0.9999992847442627f));
+  } else {
+    p = f2_fma(f2(0.0551716685295105f, 0.0551716685295105f), f,
+               f2(0.2426111251115799f, 0.2426111251115799f));
+    p = f2_fma(p, f, f2(0.6932609677314758f, 0.6932609677314758f));
+    p = f2_fma(p, f, f2(0.9999280571937561f, 0.9999280571937561f));
+  }
+  float na, nb, pa, pb;
+  f2_get(n, na, nb);
+  f2_get(p, pa, pb);
+  return f2(__uint_as_float(__float_as_uint(pa) + (__float_as_uint(na) << 23)),
+            __uint_as_float(__float_as_uint(pb) + (__float_as_uint(nb) << 23)));
+}
+
 __device__ __forceinline__ void tc_fail(unsigned* err, volatile int* abort, unsigned code) {
   *abort = 1;
   atomicCAS(err, 0u, code);
@@ -108,13 +165,53 @@ __device__ __forceinline__ void store8(const AttnArgs& a, int64_t at, const floa
   }
 }
 
+// Rows, positions and keys of a CTA's two tiles.
+struct TcGeometry {
+  int64_t row0;     // first row of the pair in q and out
+  int64_t keys;     // of the sequence
+  int64_t place0;   // position of the pair's first token
+  int64_t lo;       // first key that any row sees
+  int64_t start;    // first key of key tile 0
+  int64_t hi_all;   // one past the last key that any row sees
+  int tokens0, tokens1;  // of tile A and B
+  int tiles0, tiles1;    // key tiles of A and B
+};
+__device__ __forceinline__ int64_t tc_pairs(const TcArgs& p, const SeqSpan& sp) {
+  const int64_t rows = p.a.paged && sp.rows > p.a.max_new ? p.a.max_new : sp.rows;
+  return (rows + 2 * p.tile_tokens - 1) / (2 * p.tile_tokens);
+}
+__device__ __forceinline__ TcGeometry tc_geometry(const TcArgs& p, int seq, int64_t pair) {
+  const AttnArgs& a = p.a;
+  const SeqSpan sp = seq_span(a, seq);
+  const int64_t rows = a.paged && sp.rows > a.max_new ? a.max_new : sp.rows;
+  const int64_t tok0 = pair * 2 * p.tile_tokens, left = rows - tok0;  // left: at least 1
+  TcGeometry g;
+  g.row0 = sp.begin + tok0;
+  g.keys = sp.keys;
+  g.place0 = sp.keys - sp.rows + tok0;
+  g.tokens0 = static_cast<int>(left < p.tile_tokens ? left : p.tile_tokens);
+  g.tokens1 = static_cast<int>(left < 2 * p.tile_tokens ? left : 2 * p.tile_tokens) - g.tokens0;
+  g.lo = a.window > 0 && g.place0 - a.window + 1 > 0 ? g.place0 - a.window + 1 : 0;
+  g.start = g.lo / kKeys * kKeys;
+  int64_t hi0 = sp.keys, hi1 = sp.keys;
+  if (a.causal) {
+    const int64_t e0 = g.place0 + g.tokens0, e1 = g.place0 + p.tile_tokens + g.tokens1;
+    if (e0 < hi0) hi0 = e0;
+    if (e1 < hi1) hi1 = e1;
+  }
+  g.hi_all = g.tokens1 > 0 ? hi1 : hi0;
+  g.tiles0 = hi0 > g.lo ? static_cast<int>((hi0 - g.start + kKeys - 1) / kKeys) : 0;
+  g.tiles1 = g.tokens1 > 0 && hi1 > g.lo ? static_cast<int>((hi1 - g.start + kKeys - 1) / kKeys) : 0;
+  return g;
+}
+
 template <typename T, int DP>
 __global__ void __launch_bounds__(kTcThreads, 1)
     k_attn_tc(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
               const __grid_constant__ CUtensorMap map_v, const TcArgs p) {
   using Sh = TcShape<DP>;
   extern __shared__ uint8_t smem_raw[];
-  __shared__ uint64_t q_full, landed, s_full[2], p_full[2], o_done[2], drain;
+  __shared__ uint64_t q_full, landed, s_full[2], p_full[2][2], o_done[2], drain;
   __shared__ uint64_t kv_full[Sh::kSlots], kv_empty[Sh::kSlots];
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_word;
@@ -131,15 +228,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 
   // The CTA's pair of tiles: pairs are counted from the last sequence's last
   // tokens, so that the pairs with the most keys come first.
-  const int pair_tokens = 2 * p.tile_tokens;
-  auto pairs_of = [&](const SeqSpan& sp) {
-    const int64_t rows = a.paged && sp.rows > a.max_new ? a.max_new : sp.rows;
-    return (rows + pair_tokens - 1) / pair_tokens;
-  };
   const int per = (a.sequences + kTcThreads - 1) / kTcThreads;
   const int f0 = min(a.sequences, tid * per), f1 = min(a.sequences, f0 + per);
   int64_t mine = 0;
-  for (int s = f0; s < f1; ++s) mine += pairs_of(seq_span(a, s));
+  for (int s = f0; s < f1; ++s) mine += tc_pairs(p, seq_span(a, s));
   int64_t scan = mine;
 #pragma unroll
   for (int o = 1; o < 32; o *= 2) {
@@ -163,7 +255,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     int64_t at = before;
     int s = f0;
     while (true) {
-      const int64_t n = pairs_of(seq_span(a, s));
+      const int64_t n = tc_pairs(p, seq_span(a, s));
       if (pair < at + n) break;
       at += n;
       ++s;
@@ -178,7 +270,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     mbar_init(&drain, 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s_full[i], 1);
-      mbar_init(&p_full[i], 4);
+      mbar_init(&p_full[i][0], 4);
+      mbar_init(&p_full[i][1], 4);
       mbar_init(&o_done[i], 1);
     }
     for (int i = 0; i < Sh::kSlots; ++i) {
@@ -196,34 +289,13 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
 
-  // Rows, positions and keys of the two tiles.
   const int seq = s_seq;
-  const SeqSpan sp = seq_span(a, seq);
-  const int64_t rows_all = a.paged && sp.rows > a.max_new ? a.max_new : sp.rows;
-  const int64_t tok0 = s_pair * pair_tokens;
-  const int64_t place0 = sp.keys - sp.rows + tok0;
-  const int64_t left = rows_all - tok0;  // at least 1
-  int tokens[2];
-  tokens[0] = static_cast<int>(left < p.tile_tokens ? left : p.tile_tokens);
-  tokens[1] = static_cast<int>(left < pair_tokens ? left : pair_tokens) - tokens[0];
-  int64_t lo = 0;
-  if (a.window > 0 && place0 - a.window + 1 > 0) lo = place0 - a.window + 1;
-  const int64_t start = lo / kKeys * kKeys;
-  int64_t hi[2];
-  int tiles[2];
-#pragma unroll
-  for (int t = 0; t < 2; ++t) {
-    hi[t] = sp.keys;
-    const int64_t end = place0 + t * p.tile_tokens + tokens[t];
-    if (a.causal && end < hi[t]) hi[t] = end;
-    tiles[t] = tokens[t] > 0 && hi[t] > lo ? static_cast<int>((hi[t] - start + kKeys - 1) / kKeys)
-                                           : 0;
-  }
-  const int64_t hi_all = tokens[1] > 0 ? hi[1] : hi[0];
-  const int n_all = tiles[0] > tiles[1] ? tiles[0] : tiles[1];
+  const TcGeometry g = tc_geometry(p, seq, s_pair);
+  const int64_t lo = g.lo, start = g.start, hi_all = g.hi_all;
+  const int n_all = max(g.tiles0, g.tiles1);
   const int j0 = static_cast<int>(static_cast<int64_t>(n_all) * part / p.splits);
   const int j1 = static_cast<int>(static_cast<int64_t>(n_all) * (part + 1) / p.splits);
-  const int n0 = max(0, min(j1, tiles[0]) - j0), n1 = max(0, min(j1, tiles[1]) - j0);
+  const int n0 = max(0, min(j1, g.tiles0) - j0), n1 = max(0, min(j1, g.tiles1) - j0);
   const int n = max(n0, n1);  // key tiles of this CTA
   // Keys of tile j that some row sees: [v_lo, v_hi) of its 128.
   auto v_lo = [&](int j) {
@@ -254,7 +326,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         if ((t == 0 ? n0 : n1) == 0) continue;
         for (int h = 0; h < Sh::kHalves; ++h)
           tma_load_4d(sq + t * Sh::kTileBytes + h * 16384, &map_q, &q_full, h * 128, 0, head,
-                      static_cast<int32_t>(sp.begin + tok0 + t * p.tile_tokens));
+                      static_cast<int32_t>(g.row0 + t * p.tile_tokens));
       }
     }
     int slot = 0, landings = 0;
@@ -271,7 +343,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       const uint32_t bytes = static_cast<uint32_t>(n_load * p.box_keys * 128 * Sh::kHalves);
       const int next_page = j + 1 < j0 + n ? page_of(j + 1) : -1;
       const int32_t c2 = a.paged ? static_cast<int32_t>((kb + first) % a.page_size)
-                                 : static_cast<int32_t>(sp.begin + kb + first);
+                                 : static_cast<int32_t>(g.row0 - g.place0 + kb + first);
       const int32_t c3 = a.paged ? page : 0;
       for (int which = 0; which < 2; ++which) {
         if (!mbar_wait(&kv_empty[slot], phase ^ 1u, abort)) {
@@ -322,71 +394,82 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     }
   } else if (warp == 9) {
     // --------------------------------------------------------------- MMAs
-    if (lane == 0 && n > 0) {
+    // The whole warp walks the loop and its waits; elect.sync names the one
+    // lane that issues, which is how the compiler knows that the operands of
+    // an MMA are one thread's and moves them to the tensor core directly.
+    if (n > 0) {
       constexpr int kFmt = std::is_same<T, __half>::value ? 0 : 1;
       const int k_steps = (a.dim + 15) / 16;
       const uint32_t id_qk = make_idesc_f16(128, kKeys, kFmt, 0);
       const uint32_t id_pv = make_idesc_f16(128, k_steps * 16, kFmt, 1);
       const uint32_t q_addr = smem_u32(sq), kv_addr = smem_u32(slots);
-      auto full = [&](int i, unsigned code) {
-        const bool got = mbar_wait_poll(&kv_full[i % Sh::kSlots],
-                                        static_cast<uint32_t>((i / Sh::kSlots) & 1), abort);
-        if (!got) tc_fail(p.err, abort, code);
+      auto wait = [&](uint64_t* bar, uint32_t phase) {
+        const bool got = __all_sync(~0u, mbar_wait_poll(bar, phase, abort));
+        if (!got && lane == 0) tc_fail(p.err, abort, kDevErrMmaWait);
         return got;
+      };
+      auto full = [&](int i) {  // ring entry i has landed
+        return wait(&kv_full[i % Sh::kSlots], static_cast<uint32_t>((i / Sh::kSlots) & 1));
       };
       auto qk = [&](int t, int i) {  // key tile i of this CTA is ring entry 2 i
         const uint32_t b = kv_addr + ((2 * i) % Sh::kSlots) * Sh::kTileBytes;
         const uint32_t q = q_addr + t * Sh::kTileBytes;
-        for (int k = 0; k < k_steps; ++k) {
-          const uint32_t off = (k / 4) * 16384 + (k % 4) * 32;
-          umma_f16(tmem + Sh::kS + t * 128, make_sdesc(q + off, 16, 1024, 2),
-                   make_sdesc(b + off, 16, 1024, 2), id_qk, k > 0);
+        tc_fence_after();
+        if (elect_one()) {
+          for (int k = 0; k < k_steps; ++k) {
+            const uint32_t off = (k / 4) * 16384 + (k % 4) * 32;
+            umma_f16(tmem + Sh::kS + t * 128, make_sdesc(q + off, 16, 1024, 2),
+                     make_sdesc(b + off, 16, 1024, 2), id_qk, k > 0);
+          }
+          umma_commit(&s_full[t]);
         }
-        umma_commit(&s_full[t]);
+        __syncwarp();
       };
+      // P comes in two halves of 64 keys: the product of the first runs
+      // while the second's weights are found.
       auto pv = [&](int t, int i) {
         const uint32_t b = kv_addr + ((2 * i + 1) % Sh::kSlots) * Sh::kTileBytes;
         const int k0 = v_lo(j0 + i) / 16, k1 = (v_hi(j0 + i) + 15) / 16;
-        for (int k = k0; k < k1; ++k)
-          umma_f16_ta(tmem + Sh::kO + t * DP, tmem + Sh::kS + t * 128 + k * 8,
-                      make_sdesc(b + k * 2048, 16384, 1024, 2), id_pv, i > 0 || k > k0);
-        umma_commit(&o_done[t]);
+        for (int h = 0; h < 2; ++h) {
+          if (!wait(&p_full[t][h], static_cast<uint32_t>(i & 1))) return false;
+          tc_fence_after();
+          if (elect_one()) {
+            for (int k = max(k0, 4 * h); k < min(k1, 4 * h + 4); ++k)
+              umma_f16_ta(tmem + Sh::kO + t * DP, tmem + Sh::kS + t * 128 + k * 8,
+                          make_sdesc(b + k * 2048, 16384, 1024, 2), id_pv, i > 0 || k > k0);
+            if (h == 1) umma_commit(&o_done[t]);
+          }
+          __syncwarp();
+        }
+        return true;
       };
-      bool ok = mbar_wait_poll(&q_full, 0, abort);
-      if (!ok) tc_fail(p.err, abort, kDevErrMmaWait);
-      ok = ok && full(0, kDevErrMmaWait);
+      auto release = [&](int i) {
+        if (elect_one()) umma_commit(&kv_empty[i % Sh::kSlots]);
+        __syncwarp();
+      };
+      bool ok = wait(&q_full, 0) && full(0);
       if (ok) {
-        tc_fence_after();
         if (n0 > 0) qk(0, 0);
         if (n1 > 0) qk(1, 0);
-        umma_commit(&kv_empty[0]);
+        release(0);
       }
       for (int i = 0; i < n && ok; ++i) {
         for (int t = 0; t < 2 && ok; ++t) {
           const int nt = t == 0 ? n0 : n1;
           if (i >= nt) continue;
-          ok = mbar_wait_poll(&p_full[t], static_cast<uint32_t>(i & 1), abort);
-          if (!ok) tc_fail(p.err, abort, kDevErrMmaWait);
-          if (!ok || !(ok = full(2 * i + 1, kDevErrMmaWait))) break;
-          tc_fence_after();
-          pv(t, i);
-          if (i + 1 >= nt) continue;
-          if (!(ok = full(2 * i + 2, kDevErrMmaWait))) break;
+          ok = full(2 * i + 1) && pv(t, i);
+          if (!ok || i + 1 >= nt) continue;
           // P is read before the next S is written over it.
-          ok = mbar_wait_poll(&o_done[t], static_cast<uint32_t>(i & 1), abort);
-          if (!ok) {
-            tc_fail(p.err, abort, kDevErrMmaWait);
-            break;
-          }
-          tc_fence_after();
-          qk(t, i + 1);
+          ok = full(2 * i + 2) && wait(&o_done[t], static_cast<uint32_t>(i & 1));
+          if (ok) qk(t, i + 1);
         }
         if (!ok) break;
-        umma_commit(&kv_empty[(2 * i + 1) % Sh::kSlots]);
-        if (i + 1 < n) umma_commit(&kv_empty[(2 * i + 2) % Sh::kSlots]);
+        release(2 * i + 1);
+        if (i + 1 < n) release(2 * i + 2);
       }
       // Every MMA completes before tensor memory is freed.
-      umma_commit(&drain);
+      if (elect_one()) umma_commit(&drain);
+      __syncwarp();
       mbar_wait(&drain, 0, nullptr);
     }
     __syncwarp();
@@ -397,16 +480,27 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     const int t = warp / 4;
     const int nt = t == 0 ? n0 : n1;
     const int row = tid % 128;
+    // The row's keys [row_beg, row_end), and those that every row of the tile
+    // sees, counted from the first key tile.
+    const int64_t place = g.place0 + t * p.tile_tokens;  // of the tile's first token
     const int tok = row / p.group;
-    const bool real = tok < tokens[t];
-    const int64_t tok_t = t * p.tile_tokens;  // first token of the tile in the pair
-    const int64_t place = place0 + tok_t + tok;
+    auto end_of = [&](int64_t at) {
+      const int64_t e = a.causal && at + 1 < g.keys ? at + 1 : g.keys;
+      return static_cast<int>(e > start ? e - start : 0);
+    };
+    auto beg_of = [&](int64_t at) {
+      const int64_t b = a.window > 0 ? at - a.window + 1 : 0;
+      return static_cast<int>(b > start ? b - start : 0);
+    };
+    const int row_end = end_of(place + tok), row_beg = beg_of(place + tok);
+    const int all_end = end_of(place);
+    const int all_beg = beg_of(place + (t == 0 ? g.tokens0 : g.tokens1) - 1);
     const uint32_t lanes = static_cast<uint32_t>((warp % 4) * 32) << 16;
     const uint32_t ts = tmem + Sh::kS + t * 128 + lanes, to = tmem + Sh::kO + t * DP + lanes;
     float m = -INFINITY, l = 0.0f;
     bool ok = true;
     for (int i = 0; i < nt && ok; ++i) {
-      const int64_t kb = start + static_cast<int64_t>(j0 + i) * kKeys;
+      const int kb = (j0 + i) * kKeys;
       ok = mbar_wait(&s_full[t], static_cast<uint32_t>(i & 1), abort);
       if (!ok) {
         tc_fail(p.err, abort, kDevErrEpiWait);
@@ -414,31 +508,23 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       }
       __syncwarp();
       tc_fence_after();
-      uint32_t s[4][32];
+      uint32_t s[kKeys];
+      tmem_ld128(ts, s);
+      const bool edge = kb + kKeys > all_end || kb < all_beg;
+      if (edge) {
+        const int end = row_end - kb, beg = row_beg - kb;
 #pragma unroll
-      for (int c = 0; c < 4; ++c) tmem_ld32_nowait(ts + c * 32, s[c]);
-#pragma unroll
-      for (int c = 0; c < 4; ++c) tmem_wait_ld32(s[c]);
-      const int64_t first_place = place0 + tok_t, last_place = first_place + tokens[t] - 1;
-      if (kb + kKeys > sp.keys || (a.causal && kb + kKeys - 1 > first_place) ||
-          (a.window > 0 && kb <= last_place - a.window)) {
-        int64_t e = sp.keys, b = 0;
-        if (a.causal && place + 1 < e) e = place + 1;
-        if (a.window > 0) b = place - a.window + 1;
-        const int end = static_cast<int>(e - kb < 0 ? 0 : (e - kb > kKeys ? kKeys : e - kb));
-        const int beg = static_cast<int>(b - kb < 0 ? 0 : (b - kb > kKeys ? kKeys : b - kb));
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-#pragma unroll
-          for (int x = 0; x < 32; ++x)
-            if (c * 32 + x >= end || c * 32 + x < beg) s[c][x] = 0xFF800000u;  // -inf
+        for (int x = 0; x < kKeys; ++x)
+          if (x >= end || x < beg) s[x] = 0xFF800000u;  // -inf
       }
       float top[4];
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
-        top[c] = __uint_as_float(s[c][0]);
+        const uint32_t* q = s + 32 * c;
+        top[c] = fmaxf(__uint_as_float(q[0]), __uint_as_float(q[1]));
 #pragma unroll
-        for (int x = 1; x < 32; ++x) top[c] = fmaxf(top[c], __uint_as_float(s[c][x]));
+        for (int x = 2; x < 32; x += 2)
+          top[c] = fmaxf(fmaxf(top[c], __uint_as_float(q[x])), __uint_as_float(q[x + 1]));
       }
       const float m2 = fmaxf(m, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])));
       const bool grow = (m2 - m) * p.scale_log2 > kGrowLog2;
@@ -458,26 +544,50 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         }
       }
       const float base = m == -INFINITY ? 0.0f : m * p.scale_log2;
-      float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+      const uint64_t scale2 = f2(p.scale_log2, p.scale_log2), base2 = f2(-base, -base);
+      uint64_t sums[2] = {0, 0};
+      // kEmu of 8 pairs go to the FMA pipe, which the other exponentials
+      // (16 a clock and SM) leave idle; never in an edge tile, where a
+      // masked weight has to be exactly 0.
+      auto weights = [&](auto emu_tag) {
+        constexpr int kEmu = decltype(emu_tag)::value;
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        uint32_t w[32];
+        for (int c = 0; c < 4; ++c) {
+          uint32_t w[16];
 #pragma unroll
-        for (int x = 0; x < 32; ++x) {
-          const int c = 2 * h + x / 16, y = 2 * (x % 16);
-          const float e0 = tc_ex2(fmaf(__uint_as_float(s[c][y]), p.scale_log2, -base));
-          const float e1 = tc_ex2(fmaf(__uint_as_float(s[c][y + 1]), p.scale_log2, -base));
-          sum[x & 1] += e0;
-          sum[2 + (x & 1)] += e1;
-          w[x] = pack2<T>(e0, e1);
+          for (int x = 0; x < 16; ++x) {
+            const uint32_t* q = s + 32 * c + 2 * x;
+            uint64_t e = f2_fma(f2(__uint_as_float(q[0]), __uint_as_float(q[1])), scale2, base2);
+            float e0, e1;
+            if ((x * kEmu) % 8 < kEmu) {
+              e = f2_exp2<T>(e);
+              f2_get(e, e0, e1);
+            } else {
+              f2_get(e, e0, e1);
+              e0 = tc_ex2(e0);
+              e1 = tc_ex2(e1);
+              e = f2(e0, e1);
+            }
+            sums[x & 1] = f2_add(sums[x & 1], e);
+            w[x] = pack2<T>(e0, e1);
+          }
+          tmem_st16(ts + c * 16, w);
+          if (c & 1) {
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&p_full[t][c / 2]);
+          }
         }
-        tmem_st32(ts + h * 32, w);
-      }
-      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-      tmem_wait_st();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&p_full[t]);
+      };
+      if (edge)
+        weights(std::integral_constant<int, 0>{});
+      else
+        weights(std::integral_constant<int, kEmuPairs>{});
+      float sa, sb, sc, sd;
+      f2_get(sums[0], sa, sb);
+      f2_get(sums[1], sc, sd);
+      l += (sa + sb) + (sc + sd);
     }
     if (nt > 0 && ok) {
       ok = mbar_wait(&o_done[t], static_cast<uint32_t>((nt - 1) & 1), abort);
@@ -486,8 +596,14 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       tc_fence_after();
     }
     ok = __all_sync(~0u, ok);
-    const int64_t out_row = sp.begin + tok0 + tok_t + tok;
-    const int h = head * p.group + (row - tok * p.group);
+    // The geometry is worked out anew, from values the compiler cannot know
+    // to be the same, so that the loop above does not carry it in registers.
+    const TcGeometry e = tc_geometry(p, *const_cast<volatile int*>(&s_seq),
+                                     *const_cast<volatile int64_t*>(&s_pair));
+    const int tk = row / p.group;
+    const bool real = tk < (t == 0 ? e.tokens0 : e.tokens1);
+    const int64_t out_row = e.row0 + t * p.tile_tokens + tk;
+    const int h = head * p.group + (row - tk * p.group);
     const int64_t cta = static_cast<int64_t>(blockIdx.x);
     if (ok) {
       const float f = p.splits > 1 ? 1.0f : (l == 0.0f ? 0.0f : 1.0f / l);
@@ -538,10 +654,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         // A thread joins 4 columns of a row, all threads side by side.
         const int64_t c0 = cta - part;
         for (int u = tid; u < 256 * (DP / 4); u += 256) {
-          const int r = u / (DP / 4), e = (u % (DP / 4)) * 4;
+          const int r = u / (DP / 4), col = (u % (DP / 4)) * 4;
           const int tt = r / 128, rr = r % 128;
-          const int tk = rr / p.group;
-          if (tk >= tokens[tt]) continue;
+          const int jt = rr / p.group;
+          if (jt >= (tt == 0 ? e.tokens0 : e.tokens1)) continue;
           float mm = -INFINITY;
           for (int x = 0; x < p.splits; ++x)
             mm = fmaxf(mm, __ldcg(&p.part_ml[(c0 + x) * 256 + r].x));
@@ -553,7 +669,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             if (ml.y == 0.0f) continue;  // no key of this part counts
             const float f = tc_ex2(ml.x - bs);
             const float4 v =
-                __ldcg(reinterpret_cast<const float4*>(p.part_o + ((c0 + x) * 256 + r) * DP + e));
+                __ldcg(reinterpret_cast<const float4*>(p.part_o + ((c0 + x) * 256 + r) * DP + col));
             sum = fmaf(ml.y, f, sum);
             acc.x = fmaf(v.x, f, acc.x);
             acc.y = fmaf(v.y, f, acc.y);
@@ -561,10 +677,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             acc.w = fmaf(v.w, f, acc.w);
           }
           const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-          const int64_t orow = sp.begin + tok0 + tt * p.tile_tokens + tk;
-          const int oh = head * p.group + (rr - tk * p.group);
-          if (e < a.dim) {
-            const int64_t at = orow * a.o_token + oh * a.o_head + e;
+          const int64_t orow = e.row0 + tt * p.tile_tokens + jt;
+          const int oh = head * p.group + (rr - jt * p.group);
+          if (col < a.dim) {
+            const int64_t at = orow * a.o_token + oh * a.o_head + col;
             const float v[4] = {acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv};
             if (a.out_dtype == PSPML_DTYPE_S8) {
               char4 c;
@@ -578,7 +694,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                   make_uint2(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]));
             }
           }
-          if (e == 0 && a.lse != nullptr)
+          if (col == 0 && a.lse != nullptr)
             a.lse[orow * a.q_heads + oh] =
                 sum == 0.0f ? -INFINITY : (log2f(sum) + bs) * 0.69314718055994531f;
         }
