@@ -403,69 +403,85 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       const uint32_t id_qk = make_idesc_f16(128, kKeys, kFmt, 0);
       const uint32_t id_pv = make_idesc_f16(128, k_steps * 16, kFmt, 1);
       const uint32_t q_addr = smem_u32(sq), kv_addr = smem_u32(slots);
+      const int k_first = v_lo(j0) / 16;                  // steps of the first key tile
+      const int k_last = (v_hi(j0 + n - 1) + 15) / 16;    // and of the last
       auto wait = [&](uint64_t* bar, uint32_t phase) {
         const bool got = __all_sync(~0u, mbar_wait_poll(bar, phase, abort));
         if (!got && lane == 0) tc_fail(p.err, abort, kDevErrMmaWait);
         return got;
       };
-      auto full = [&](int i) {  // ring entry i has landed
-        return wait(&kv_full[i % Sh::kSlots], static_cast<uint32_t>((i / Sh::kSlots) & 1));
-      };
-      auto qk = [&](int t, int i) {  // key tile i of this CTA is ring entry 2 i
-        const uint32_t b = kv_addr + ((2 * i) % Sh::kSlots) * Sh::kTileBytes;
-        const uint32_t q = q_addr + t * Sh::kTileBytes;
+      // Descriptors are built once a tile; a step adds its 16-byte units to
+      // the address, which stays within its 14 bits.  `freed`: the slot
+      // whose last reader this product is.
+      auto qk = [&](int t, int slot, uint64_t* freed) {
         tc_fence_after();
         if (elect_one()) {
-          for (int k = 0; k < k_steps; ++k) {
-            const uint32_t off = (k / 4) * 16384 + (k % 4) * 32;
-            umma_f16(tmem + Sh::kS + t * 128, make_sdesc(q + off, 16, 1024, 2),
-                     make_sdesc(b + off, 16, 1024, 2), id_qk, k > 0);
+          const uint64_t q = make_sdesc(q_addr + t * Sh::kTileBytes, 16, 1024, 2);
+          const uint64_t b = make_sdesc(kv_addr + slot * Sh::kTileBytes, 16, 1024, 2);
+#pragma unroll
+          for (int k = 0; k < DP / 16; ++k) {
+            const int off = (k / 4) * 1024 + (k % 4) * 2;
+            if (k < k_steps)
+              umma_f16(tmem + Sh::kS + t * 128, q + off, b + off, id_qk, k > 0 ? 1u : 0u);
           }
           umma_commit(&s_full[t]);
+          if (freed != nullptr) umma_commit(freed);
         }
         __syncwarp();
       };
       // P comes in two halves of 64 keys: the product of the first runs
       // while the second's weights are found.
-      auto pv = [&](int t, int i) {
-        const uint32_t b = kv_addr + ((2 * i + 1) % Sh::kSlots) * Sh::kTileBytes;
-        const int k0 = v_lo(j0 + i) / 16, k1 = (v_hi(j0 + i) + 15) / 16;
+      auto pv = [&](int t, int i, int slot, uint64_t* freed) {
+        const int k0 = i == 0 ? k_first : 0, k1 = i == n - 1 ? k_last : kKeys / 16;
+#pragma unroll
         for (int h = 0; h < 2; ++h) {
           if (!wait(&p_full[t][h], static_cast<uint32_t>(i & 1))) return false;
           tc_fence_after();
           if (elect_one()) {
-            for (int k = max(k0, 4 * h); k < min(k1, 4 * h + 4); ++k)
-              umma_f16_ta(tmem + Sh::kO + t * DP, tmem + Sh::kS + t * 128 + k * 8,
-                          make_sdesc(b + k * 2048, 16384, 1024, 2), id_pv, i > 0 || k > k0);
-            if (h == 1) umma_commit(&o_done[t]);
+            const uint64_t b = make_sdesc(kv_addr + slot * Sh::kTileBytes, 16384, 1024, 2);
+            const uint32_t o = tmem + Sh::kO + t * DP, a = tmem + Sh::kS + t * 128;
+#pragma unroll
+            for (int k = 4 * h; k < 4 * h + 4; ++k)
+              if (k >= k0 && k < k1)
+                umma_f16_ta(o, a + k * 8, b + k * 128, id_pv, i > 0 || k > k0 ? 1u : 0u);
+            if (h == 1) {
+              umma_commit(&o_done[t]);
+              if (freed != nullptr) umma_commit(freed);
+            }
           }
           __syncwarp();
         }
         return true;
       };
-      auto release = [&](int i) {
-        if (elect_one()) umma_commit(&kv_empty[i % Sh::kSlots]);
-        __syncwarp();
-      };
-      bool ok = wait(&q_full, 0) && full(0);
+      bool ok = wait(&q_full, 0) && wait(&kv_full[0], 0);
       if (ok) {
-        if (n0 > 0) qk(0, 0);
-        if (n1 > 0) qk(1, 0);
-        release(0);
+        if (n0 > 0) qk(0, 0, n1 > 0 ? nullptr : &kv_empty[0]);
+        if (n1 > 0) qk(1, 0, &kv_empty[0]);
       }
+      int v_slot = 1, k_slot = 2;  // ring slots of value tile i and key tile i + 1
+      uint32_t v_phase = 0, k_phase = 0;
       for (int i = 0; i < n && ok; ++i) {
-        for (int t = 0; t < 2 && ok; ++t) {
-          const int nt = t == 0 ? n0 : n1;
-          if (i >= nt) continue;
-          ok = full(2 * i + 1) && pv(t, i);
+        ok = wait(&kv_full[v_slot], v_phase);
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          const int nt = t == 0 ? n0 : n1, other = t == 0 ? n1 : 0;
+          if (!ok || i >= nt) continue;
+          ok = pv(t, i, v_slot, i < other ? nullptr : &kv_empty[v_slot]);
           if (!ok || i + 1 >= nt) continue;
           // P is read before the next S is written over it.
-          ok = full(2 * i + 2) && wait(&o_done[t], static_cast<uint32_t>(i & 1));
-          if (ok) qk(t, i + 1);
+          ok = wait(&kv_full[k_slot], k_phase) && wait(&o_done[t], static_cast<uint32_t>(i & 1));
+          if (ok) qk(t, k_slot, i + 1 < other ? nullptr : &kv_empty[k_slot]);
         }
-        if (!ok) break;
-        release(2 * i + 1);
-        if (i + 1 < n) release(2 * i + 2);
+        v_slot += 2;
+        if (v_slot >= Sh::kSlots) {
+          v_slot -= Sh::kSlots;
+          v_phase ^= 1u;
+        }
+        k_slot += 2;
+        if (k_slot >= Sh::kSlots) {
+          k_slot -= Sh::kSlots;
+          k_phase ^= 1u;
+        }
       }
       // Every MMA completes before tensor memory is freed.
       if (elect_one()) umma_commit(&drain);
