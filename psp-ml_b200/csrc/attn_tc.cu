@@ -405,10 +405,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       const uint32_t q_addr = smem_u32(sq), kv_addr = smem_u32(slots);
       const int k_first = v_lo(j0) / 16;                  // steps of the first key tile
       const int k_last = (v_hi(j0 + n - 1) + 15) / 16;    // and of the last
+      // A wait that gives up only raises the abort flag, after which every
+      // other wait ends at once; the flag is looked at once a key tile.
       auto wait = [&](uint64_t* bar, uint32_t phase) {
-        const bool got = __all_sync(~0u, mbar_wait_poll(bar, phase, abort));
-        if (!got && lane == 0) tc_fail(p.err, abort, kDevErrMmaWait);
-        return got;
+        if (!mbar_wait_poll(bar, phase, abort)) tc_fail(p.err, abort, kDevErrMmaWait);
+        __syncwarp();
       };
       // Descriptors are built once a tile; a step adds its 16-byte units to
       // the address, which stays within its 14 bits.  `freed`: the slot
@@ -435,7 +436,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         const int k0 = i == 0 ? k_first : 0, k1 = i == n - 1 ? k_last : kKeys / 16;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          if (!wait(&p_full[t][h], static_cast<uint32_t>(i & 1))) return false;
+          wait(&p_full[t][h], static_cast<uint32_t>(i & 1));
           tc_fence_after();
           if (elect_one()) {
             const uint64_t b = make_sdesc(kv_addr + slot * Sh::kTileBytes, 16384, 1024, 2);
@@ -451,26 +452,26 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           }
           __syncwarp();
         }
-        return true;
       };
-      bool ok = wait(&q_full, 0) && wait(&kv_full[0], 0);
-      if (ok) {
-        if (n0 > 0) qk(0, 0, n1 > 0 ? nullptr : &kv_empty[0]);
-        if (n1 > 0) qk(1, 0, &kv_empty[0]);
-      }
+      wait(&q_full, 0);
+      wait(&kv_full[0], 0);
+      if (n0 > 0) qk(0, 0, n1 > 0 ? nullptr : &kv_empty[0]);
+      if (n1 > 0) qk(1, 0, &kv_empty[0]);
       int v_slot = 1, k_slot = 2;  // ring slots of value tile i and key tile i + 1
       uint32_t v_phase = 0, k_phase = 0;
-      for (int i = 0; i < n && ok; ++i) {
-        ok = wait(&kv_full[v_slot], v_phase);
+      for (int i = 0; i < n; ++i) {
+        if (__any_sync(~0u, *abort)) break;
+        wait(&kv_full[v_slot], v_phase);
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
           const int nt = t == 0 ? n0 : n1, other = t == 0 ? n1 : 0;
-          if (!ok || i >= nt) continue;
-          ok = pv(t, i, v_slot, i < other ? nullptr : &kv_empty[v_slot]);
-          if (!ok || i + 1 >= nt) continue;
+          if (i >= nt) continue;
+          pv(t, i, v_slot, i < other ? nullptr : &kv_empty[v_slot]);
+          if (i + 1 >= nt) continue;
+          wait(&kv_full[k_slot], k_phase);
           // P is read before the next S is written over it.
-          ok = wait(&kv_full[k_slot], k_phase) && wait(&o_done[t], static_cast<uint32_t>(i & 1));
-          if (ok) qk(t, k_slot, i + 1 < other ? nullptr : &kv_empty[k_slot]);
+          wait(&o_done[t], static_cast<uint32_t>(i & 1));
+          qk(t, k_slot, i + 1 < other ? nullptr : &kv_empty[k_slot]);
         }
         v_slot += 2;
         if (v_slot >= Sh::kSlots) {
