@@ -53,6 +53,7 @@ constexpr int kSoftmaxRegs = 200;
 constexpr int kOtherRegs = 104;
 constexpr int kTcWarps = kTcThreads / 32;
 constexpr int kKeys = 128;        // keys a tile
+constexpr int kPieces = 2;        // in which P is handed to the MMA warp
 constexpr int kEmuPairs = 0;      // of 8 pairs of exponentials, those on the FMA pipe
 constexpr float kGrowLog2 = 8.0f; // largest stale maximum, as a power of two
 
@@ -211,7 +212,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
               const __grid_constant__ CUtensorMap map_v, const TcArgs p) {
   using Sh = TcShape<DP>;
   extern __shared__ uint8_t smem_raw[];
-  __shared__ uint64_t q_full, landed, s_full[2], p_full[2][2], o_done[2], drain;
+  __shared__ uint64_t q_full, landed, s_full[2], p_full[2][kPieces], o_done[2], drain;
   __shared__ uint64_t kv_full[Sh::kSlots], kv_empty[Sh::kSlots];
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_word;
@@ -270,8 +271,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     mbar_init(&drain, 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s_full[i], 1);
-      mbar_init(&p_full[i][0], 4);
-      mbar_init(&p_full[i][1], 4);
+      for (int h = 0; h < kPieces; ++h) mbar_init(&p_full[i][h], 4);
       mbar_init(&o_done[i], 1);
     }
     for (int i = 0; i < Sh::kSlots; ++i) {
@@ -406,7 +406,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       const int k_first = v_lo(j0) / 16;                  // steps of the first key tile
       const int k_last = (v_hi(j0 + n - 1) + 15) / 16;    // and of the last
       // A wait that gives up only raises the abort flag, after which every
-      // other wait ends at once; the flag is looked at once a key tile.
+      // other wait ends at once; the flag is looked at now and then.
       auto wait = [&](uint64_t* bar, uint32_t phase) {
         if (!mbar_wait_poll(bar, phase, abort)) tc_fail(p.err, abort, kDevErrMmaWait);
         __syncwarp();
@@ -430,22 +430,22 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         }
         __syncwarp();
       };
-      // P comes in two halves of 64 keys: the product of the first runs
-      // while the second's weights are found.
+      // P comes in pieces: the product of one runs while the next one's
+      // weights are found.
       auto pv = [&](int t, int i, int slot, uint64_t* freed) {
         const int k0 = i == 0 ? k_first : 0, k1 = i == n - 1 ? k_last : kKeys / 16;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
+        for (int h = 0; h < kPieces; ++h) {
           wait(&p_full[t][h], static_cast<uint32_t>(i & 1));
           tc_fence_after();
           if (elect_one()) {
             const uint64_t b = make_sdesc(kv_addr + slot * Sh::kTileBytes, 16384, 1024, 2);
             const uint32_t o = tmem + Sh::kO + t * DP, a = tmem + Sh::kS + t * 128;
 #pragma unroll
-            for (int k = 4 * h; k < 4 * h + 4; ++k)
+            for (int k = h * (8 / kPieces); k < (h + 1) * (8 / kPieces); ++k)
               if (k >= k0 && k < k1)
                 umma_f16_ta(o, a + k * 8, b + k * 128, id_pv, i > 0 || k > k0 ? 1u : 0u);
-            if (h == 1) {
+            if (h == kPieces - 1) {
               umma_commit(&o_done[t]);
               if (freed != nullptr) umma_commit(freed);
             }
@@ -460,15 +460,15 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       int v_slot = 1, k_slot = 2;  // ring slots of value tile i and key tile i + 1
       uint32_t v_phase = 0, k_phase = 0;
       for (int i = 0; i < n; ++i) {
-        if (__any_sync(~0u, *abort)) break;
+        if ((i & 7) == 7 && __any_sync(~0u, *abort)) break;
         wait(&kv_full[v_slot], v_phase);
+        if (i + 1 < n) wait(&kv_full[k_slot], k_phase);
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
           const int nt = t == 0 ? n0 : n1, other = t == 0 ? n1 : 0;
           if (i >= nt) continue;
           pv(t, i, v_slot, i < other ? nullptr : &kv_empty[v_slot]);
           if (i + 1 >= nt) continue;
-          wait(&kv_full[k_slot], k_phase);
           // P is read before the next S is written over it.
           wait(&o_done[t], static_cast<uint32_t>(i & 1));
           qk(t, k_slot, i + 1 < other ? nullptr : &kv_empty[k_slot]);
@@ -589,11 +589,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             w[x] = pack2<T>(e0, e1);
           }
           tmem_st16(ts + c * 16, w);
-          if (c & 1) {
+          if ((c + 1) % (4 / kPieces) == 0) {
             tmem_wait_st();
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&p_full[t][c / 2]);
+            if (lane == 0) mbar_arrive(&p_full[t][c / (4 / kPieces)]);
           }
         }
       };
