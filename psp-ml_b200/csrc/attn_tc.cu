@@ -144,6 +144,19 @@ __device__ __forceinline__ void tc_fail(unsigned* err, volatile int* abort, unsi
   atomicCAS(err, 0u, code);
 }
 
+// Piece h of tile t's P is handed from its four softmax warps to the MMA warp
+// at a hardware barrier: polls of an mbarrier would take issue slots from the
+// two softmax warps on the MMA warp's scheduler, which set the pace (2121 us
+// against 1854 at 16384 tokens and 32 heads with tight and with rare polls).
+// Both sides walk all their key tiles whatever happens, so neither waits for
+// an arrival that does not come.
+__device__ __forceinline__ void prob_arrive(int t, int h) {
+  asm volatile("bar.arrive %0, 160;" ::"r"(2 + t * kPieces + h) : "memory");
+}
+__device__ __forceinline__ void prob_wait(int t, int h) {
+  asm volatile("bar.sync %0, 160;" ::"r"(2 + t * kPieces + h) : "memory");
+}
+
 // Eight neighbouring outputs of a row.
 template <typename T>
 __device__ __forceinline__ void store8(const AttnArgs& a, int64_t at, const float* v) {
@@ -212,7 +225,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
               const __grid_constant__ CUtensorMap map_v, const TcArgs p) {
   using Sh = TcShape<DP>;
   extern __shared__ uint8_t smem_raw[];
-  __shared__ uint64_t q_full, landed, s_full[2], p_full[2][kPieces], o_done[2], drain;
+  __shared__ uint64_t q_full, landed, s_full[2], o_done[2], drain;
   __shared__ uint64_t kv_full[Sh::kSlots], kv_empty[Sh::kSlots];
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_word;
@@ -271,7 +284,6 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     mbar_init(&drain, 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s_full[i], 1);
-      for (int h = 0; h < kPieces; ++h) mbar_init(&p_full[i][h], 4);
       mbar_init(&o_done[i], 1);
     }
     for (int i = 0; i < Sh::kSlots; ++i) {
@@ -406,7 +418,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       const int k_first = v_lo(j0) / 16;                  // steps of the first key tile
       const int k_last = (v_hi(j0 + n - 1) + 15) / 16;    // and of the last
       // A wait that gives up only raises the abort flag, after which every
-      // other wait ends at once; the flag is looked at now and then.
+      // other wait ends at once.
       auto wait = [&](uint64_t* bar, uint32_t phase) {
         if (!mbar_wait_poll(bar, phase, abort)) tc_fail(p.err, abort, kDevErrMmaWait);
         __syncwarp();
@@ -436,7 +448,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         const int k0 = i == 0 ? k_first : 0, k1 = i == n - 1 ? k_last : kKeys / 16;
 #pragma unroll
         for (int h = 0; h < kPieces; ++h) {
-          wait(&p_full[t][h], static_cast<uint32_t>(i & 1));
+          prob_wait(t, h);
           tc_fence_after();
           if (elect_one()) {
             const uint64_t b = make_sdesc(kv_addr + slot * Sh::kTileBytes, 16384, 1024, 2);
@@ -460,7 +472,6 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       int v_slot = 1, k_slot = 2;  // ring slots of value tile i and key tile i + 1
       uint32_t v_phase = 0, k_phase = 0;
       for (int i = 0; i < n; ++i) {
-        if ((i & 7) == 7 && __any_sync(~0u, *abort)) break;
         wait(&kv_full[v_slot], v_phase);
         if (i + 1 < n) wait(&kv_full[k_slot], k_phase);
 #pragma unroll
@@ -516,12 +527,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     const uint32_t ts = tmem + Sh::kS + t * 128 + lanes, to = tmem + Sh::kO + t * DP + lanes;
     float m = -INFINITY, l = 0.0f;
     bool ok = true;
-    for (int i = 0; i < nt && ok; ++i) {
+    for (int i = 0; i < nt; ++i) {
       const int kb = (j0 + i) * kKeys;
-      ok = mbar_wait(&s_full[t], static_cast<uint32_t>(i & 1), abort);
-      if (!ok) {
+      if (!mbar_wait(&s_full[t], static_cast<uint32_t>(i & 1), abort)) {
         tc_fail(p.err, abort, kDevErrEpiWait);
-        break;
+        ok = false;
       }
       __syncwarp();
       tc_fence_after();
@@ -592,8 +602,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           if ((c + 1) % (4 / kPieces) == 0) {
             tmem_wait_st();
             tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&p_full[t][c / (4 / kPieces)]);
+            prob_arrive(t, c / (4 / kPieces));
           }
         }
       };
