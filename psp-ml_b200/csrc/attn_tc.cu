@@ -51,15 +51,14 @@ namespace {
 constexpr int kTcThreads = 384;
 constexpr int kSoftmaxRegs = 200;
 constexpr int kOtherRegs = 104;
-constexpr int kTcWarps = kTcThreads / 32;
 constexpr int kKeys = 128;        // keys a tile
 constexpr int kPieces = 2;        // in which P is handed to the MMA warp
-constexpr int kEmuPairs = 0;      // of 8 pairs of exponentials, those on the FMA pipe
+constexpr int kPartsPerSm = 2;
 constexpr float kGrowLog2 = 8.0f; // largest stale maximum, as a power of two
 
 struct TcArgs {
   AttnArgs a;
-  float* part_o;       // [ctas][256][DP]
+  float4* part_o;      // [ctas][DP / 4][256]: a warp's rows side by side
   float2* part_ml;     // [ctas][256]
   unsigned* arrived;   // [segments]
   unsigned* err;
@@ -102,41 +101,6 @@ __device__ __forceinline__ uint64_t f2_add(uint64_t a, uint64_t b) {
   uint64_t r;
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
-}
-
-// 2^x of two floats in [-inf, 127) on the FMA pipe: x = n + f with n the
-// nearest integer (found by adding 1.5 * 2^23, whose low bits then hold n),
-// 2^f by the polynomial of least relative error on [-1/2, 1/2] (fitted by
-// exchange; 2^-13.7 of degree 3 for BF16 weights, 2^-18.5 of degree 4 for
-// F16, a sixteenth of their rounding or less), n added to the exponent.  x
-// is cut at -126.
-template <typename T>
-__device__ __forceinline__ uint64_t f2_exp2(uint64_t x) {
-  float a, b;
-  f2_get(x, a, b);
-  x = f2(fmaxf(a, -126.0f), fmaxf(b, -126.0f));
-  const uint64_t magic = f2(12582912.0f, 12582912.0f);
-  const uint64_t n = f2_add(x, magic);
-  const uint64_t r = f2_add(n, f2(-12582912.0f, -12582912.0f));
-  const uint64_t f = f2_fma(r, f2(-1.0f, -1.0f), x);
-  uint64_t p;
-  if constexpr (std::is_same<T, __half>::value) {
-    p = f2_fma(f2(0.009570102207362652f, 0.009570102207362652f), f,
-               f2(0.05591785907745361f, 0.05591785907745361f));
-    p = f2_fma(p, f, f2(0.240247443318367f, 0.240247443318367f));
-    p = f2_fma(p, f, f2(0.6931217908859253f, 0.6931217908859253f));
-    p = f2_fma(p, f, f2(0.9999992847442627f, 0.9999992847442627f));
-  } else {
-    p = f2_fma(f2(0.0551716685295105f, 0.0551716685295105f), f,
-               f2(0.2426111251115799f, 0.2426111251115799f));
-    p = f2_fma(p, f, f2(0.6932609677314758f, 0.6932609677314758f));
-    p = f2_fma(p, f, f2(0.9999280571937561f, 0.9999280571937561f));
-  }
-  float na, nb, pa, pb;
-  f2_get(n, na, nb);
-  f2_get(p, pa, pb);
-  return f2(__uint_as_float(__float_as_uint(pa) + (__float_as_uint(na) << 23)),
-            __uint_as_float(__float_as_uint(pb) + (__float_as_uint(nb) << 23)));
 }
 
 __device__ __forceinline__ void tc_fail(unsigned* err, volatile int* abort, unsigned code) {
@@ -190,13 +154,44 @@ struct TcGeometry {
   int tokens0, tokens1;  // of tile A and B
   int tiles0, tiles1;    // key tiles of A and B
 };
-__device__ __forceinline__ int64_t tc_pairs(const TcArgs& p, const SeqSpan& sp) {
-  const int64_t rows = p.a.paged && sp.rows > p.a.max_new ? p.a.max_new : sp.rows;
-  return (rows + 2 * p.tile_tokens - 1) / (2 * p.tile_tokens);
+// Pair `idx` of the call, found by one warp: the sequences' pairs are counted
+// 32 sequences at a time.  Within a sequence the last tokens come first, so
+// that the pairs with the most keys start first.  False past the last pair.
+__device__ __forceinline__ bool tc_locate(const TcArgs& p, int64_t idx, int lane, int* seq,
+                                          int64_t* pair, SeqSpan* span) {
+  const unsigned pair_tokens = 2u * p.tile_tokens;
+  for (int s0 = 0; s0 < p.a.sequences; s0 += 32) {
+    const int s = s0 + lane;
+    SeqSpan sp{0, 0, 0};
+    unsigned mine = 0;
+    if (s < p.a.sequences) {
+      sp = seq_span(p.a, s);
+      const int64_t rows = p.a.paged && sp.rows > p.a.max_new ? p.a.max_new : sp.rows;
+      mine = (static_cast<unsigned>(rows) + pair_tokens - 1) / pair_tokens;
+    }
+    unsigned scan = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o *= 2) {
+      const unsigned v = __shfl_up_sync(~0u, scan, o);
+      if (lane >= o) scan += v;
+    }
+    const unsigned all = __shfl_sync(~0u, scan, 31);
+    if (idx < all) {
+      const int at = __ffs(__ballot_sync(~0u, idx < scan)) - 1;
+      *seq = s0 + at;
+      *pair = static_cast<int64_t>(__shfl_sync(~0u, scan, at)) - 1 - idx;
+      span->begin = __shfl_sync(~0u, sp.begin, at);
+      span->keys = __shfl_sync(~0u, sp.keys, at);
+      span->rows = __shfl_sync(~0u, sp.rows, at);
+      return true;
+    }
+    idx -= all;
+  }
+  return false;
 }
-__device__ __forceinline__ TcGeometry tc_geometry(const TcArgs& p, int seq, int64_t pair) {
+__device__ __forceinline__ TcGeometry tc_geometry(const TcArgs& p, const SeqSpan& sp,
+                                                  int64_t pair) {
   const AttnArgs& a = p.a;
-  const SeqSpan sp = seq_span(a, seq);
   const int64_t rows = a.paged && sp.rows > a.max_new ? a.max_new : sp.rows;
   const int64_t tok0 = pair * 2 * p.tile_tokens, left = rows - tok0;  // left: at least 1
   TcGeometry g;
@@ -229,9 +224,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   __shared__ uint64_t kv_full[Sh::kSlots], kv_empty[Sh::kSlots];
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_word;
-  __shared__ int64_t s_sum[kTcWarps];
-  __shared__ int s_seq;
-  __shared__ int64_t s_pair;
+  __shared__ int64_t s_row0;
+  __shared__ int s_tokens[2];
   __shared__ int s_last;
   const AttnArgs& a = p.a;
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
@@ -240,44 +234,23 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   uint8_t* sq = smem;
   uint8_t* slots = smem + 2 * Sh::kTileBytes;
 
-  // The CTA's pair of tiles: pairs are counted from the last sequence's last
-  // tokens, so that the pairs with the most keys come first.
-  const int per = (a.sequences + kTcThreads - 1) / kTcThreads;
-  const int f0 = min(a.sequences, tid * per), f1 = min(a.sequences, f0 + per);
-  int64_t mine = 0;
-  for (int s = f0; s < f1; ++s) mine += tc_pairs(p, seq_span(a, s));
-  int64_t scan = mine;
-#pragma unroll
-  for (int o = 1; o < 32; o *= 2) {
-    const int64_t v = __shfl_up_sync(~0u, scan, o);
-    if (lane >= o) scan += v;
-  }
-  if (lane == 31) s_sum[warp] = scan;
-  __syncthreads();
-  int64_t total = 0, before = scan - mine;
-#pragma unroll
-  for (int w = 0; w < kTcWarps; ++w) {
-    if (w < warp) before += s_sum[w];
-    total += s_sum[w];
-  }
   const int part = static_cast<int>(blockIdx.x % p.splits);
   const int64_t seg = blockIdx.x / p.splits;
   const int head = static_cast<int>(seg % a.kv_heads);
-  const int64_t pair = total - 1 - seg / a.kv_heads;
-  if (pair < 0) return;
-  if (pair >= before && pair < before + mine) {
-    int64_t at = before;
-    int s = f0;
-    while (true) {
-      const int64_t n = tc_pairs(p, seq_span(a, s));
-      if (pair < at + n) break;
-      at += n;
-      ++s;
-    }
-    s_seq = s;
-    s_pair = pair - at;
+  int seq;
+  int64_t pair;
+  SeqSpan span;
+  if (!tc_locate(p, seg / a.kv_heads, lane, &seq, &pair, &span)) return;
+  if (warp == 8 && lane == 0) {
+    tma_prefetch_desc(&map_q);
+    tma_prefetch_desc(&map_k);
+    tma_prefetch_desc(&map_v);
   }
   if (tid == 0) {
+    const TcGeometry g = tc_geometry(p, span, pair);
+    s_row0 = g.row0;
+    s_tokens[0] = g.tokens0;
+    s_tokens[1] = g.tokens1;
     abort_word = 0;
     mbar_init(&q_full, 1);
     mbar_init(&landed, 1);
@@ -301,8 +274,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
 
-  const int seq = s_seq;
-  const TcGeometry g = tc_geometry(p, seq, s_pair);
+  const TcGeometry g = tc_geometry(p, span, pair);
   const int64_t lo = g.lo, start = g.start, hi_all = g.hi_all;
   const int n_all = max(g.tiles0, g.tiles1);
   const int j0 = static_cast<int>(static_cast<int64_t>(n_all) * part / p.splits);
@@ -573,43 +545,26 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       const float base = m == -INFINITY ? 0.0f : m * p.scale_log2;
       const uint64_t scale2 = f2(p.scale_log2, p.scale_log2), base2 = f2(-base, -base);
       uint64_t sums[2] = {0, 0};
-      // kEmu of 8 pairs go to the FMA pipe, which the other exponentials
-      // (16 a clock and SM) leave idle; never in an edge tile, where a
-      // masked weight has to be exactly 0.
-      auto weights = [&](auto emu_tag) {
-        constexpr int kEmu = decltype(emu_tag)::value;
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          uint32_t w[16];
+      for (int c = 0; c < 4; ++c) {
+        uint32_t w[16];
 #pragma unroll
-          for (int x = 0; x < 16; ++x) {
-            const uint32_t* q = s + 32 * c + 2 * x;
-            uint64_t e = f2_fma(f2(__uint_as_float(q[0]), __uint_as_float(q[1])), scale2, base2);
-            float e0, e1;
-            if ((x * kEmu) % 8 < kEmu) {
-              e = f2_exp2<T>(e);
-              f2_get(e, e0, e1);
-            } else {
-              f2_get(e, e0, e1);
-              e0 = tc_ex2(e0);
-              e1 = tc_ex2(e1);
-              e = f2(e0, e1);
-            }
-            sums[x & 1] = f2_add(sums[x & 1], e);
-            w[x] = pack2<T>(e0, e1);
-          }
-          tmem_st16(ts + c * 16, w);
-          if ((c + 1) % (4 / kPieces) == 0) {
-            tmem_wait_st();
-            tc_fence_before();
-            prob_arrive(t, c / (4 / kPieces));
-          }
+        for (int x = 0; x < 16; ++x) {
+          const uint32_t* q = s + 32 * c + 2 * x;
+          float e0, e1;
+          f2_get(f2_fma(f2(__uint_as_float(q[0]), __uint_as_float(q[1])), scale2, base2), e0, e1);
+          e0 = tc_ex2(e0);
+          e1 = tc_ex2(e1);
+          sums[x & 1] = f2_add(sums[x & 1], f2(e0, e1));
+          w[x] = pack2<T>(e0, e1);
         }
-      };
-      if (edge)
-        weights(std::integral_constant<int, 0>{});
-      else
-        weights(std::integral_constant<int, kEmuPairs>{});
+        tmem_st16(ts + c * 16, w);
+        if ((c + 1) % (4 / kPieces) == 0) {
+          tmem_wait_st();
+          tc_fence_before();
+          prob_arrive(t, c / (4 / kPieces));
+        }
+      }
       float sa, sb, sc, sd;
       f2_get(sums[0], sa, sb);
       f2_get(sums[1], sc, sd);
@@ -622,13 +577,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       tc_fence_after();
     }
     ok = __all_sync(~0u, ok);
-    // The geometry is worked out anew, from values the compiler cannot know
-    // to be the same, so that the loop above does not carry it in registers.
-    const TcGeometry e = tc_geometry(p, *const_cast<volatile int*>(&s_seq),
-                                     *const_cast<volatile int64_t*>(&s_pair));
+    // Read back here so that the loop above does not carry them in registers.
+    const int64_t row0 = *const_cast<volatile int64_t*>(&s_row0);
     const int tk = row / p.group;
-    const bool real = tk < (t == 0 ? e.tokens0 : e.tokens1);
-    const int64_t out_row = e.row0 + t * p.tile_tokens + tk;
+    const bool real = tk < *const_cast<volatile int*>(&s_tokens[t]);
+    const int64_t out_row = row0 + t * p.tile_tokens + tk;
     const int h = head * p.group + (row - tk * p.group);
     const int64_t cta = static_cast<int64_t>(blockIdx.x);
     if (ok) {
@@ -652,11 +605,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             for (int x = 0; x < 32; x += 8)
               if (c * 32 + x < a.dim) store8<T>(a, at + c * 32 + x, v + x);
           } else {
-            float4* dst = reinterpret_cast<float4*>(p.part_o + (cta * 256 + t * 128 + row) * DP +
-                                                    c * 32);
+            float4* dst = p.part_o + (cta * (DP / 4) + c * 8) * 256 + t * 128 + row;
 #pragma unroll
             for (int x = 0; x < 8; ++x)
-              dst[x] = make_float4(v[4 * x], v[4 * x + 1], v[4 * x + 2], v[4 * x + 3]);
+              dst[x * 256] = make_float4(v[4 * x], v[4 * x + 1], v[4 * x + 2], v[4 * x + 3]);
           }
         }
       }
@@ -677,50 +629,57 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       asm volatile("bar.sync 1, 256;" ::: "memory");
       if (s_last) {
         __threadfence();
-        // A thread joins 4 columns of a row, all threads side by side.
+        // Each thread joins a row: its maximum and sum over the parts, then
+        // its columns, kCols at a time.  A part without a key that counts
+        // (sum 0) has nothing to add.
         const int64_t c0 = cta - part;
-        for (int u = tid; u < 256 * (DP / 4); u += 256) {
-          const int r = u / (DP / 4), col = (u % (DP / 4)) * 4;
-          const int tt = r / 128, rr = r % 128;
-          const int jt = rr / p.group;
-          if (jt >= (tt == 0 ? e.tokens0 : e.tokens1)) continue;
-          float mm = -INFINITY;
-          for (int x = 0; x < p.splits; ++x)
-            mm = fmaxf(mm, __ldcg(&p.part_ml[(c0 + x) * 256 + r].x));
-          const float bs = mm == -INFINITY ? 0.0f : mm;
-          float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-          float sum = 0.0f;
+        const int tt = tid / 128, rr = tid % 128;
+        const int jt = rr / p.group;
+        if (jt < s_tokens[tt]) {
+          float mm = -INFINITY, sum = 0.0f;
+#pragma unroll 4
           for (int x = 0; x < p.splits; ++x) {
-            const float2 ml = __ldcg(p.part_ml + (c0 + x) * 256 + r);
-            if (ml.y == 0.0f) continue;  // no key of this part counts
-            const float f = tc_ex2(ml.x - bs);
-            const float4 v =
-                __ldcg(reinterpret_cast<const float4*>(p.part_o + ((c0 + x) * 256 + r) * DP + col));
-            sum = fmaf(ml.y, f, sum);
-            acc.x = fmaf(v.x, f, acc.x);
-            acc.y = fmaf(v.y, f, acc.y);
-            acc.z = fmaf(v.z, f, acc.z);
-            acc.w = fmaf(v.w, f, acc.w);
+            const float2 ml = __ldcg(p.part_ml + (c0 + x) * 256 + tid);
+            const float top = fmaxf(mm, ml.x);
+            const float bs = top == -INFINITY ? 0.0f : top;
+            sum = sum * tc_ex2(mm - bs) + ml.y * tc_ex2(ml.x - bs);
+            mm = top;
           }
+          const float bs = mm == -INFINITY ? 0.0f : mm;
           const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-          const int64_t orow = e.row0 + tt * p.tile_tokens + jt;
+          const int64_t orow = row0 + tt * p.tile_tokens + jt;
           const int oh = head * p.group + (rr - jt * p.group);
-          if (col < a.dim) {
-            const int64_t at = orow * a.o_token + oh * a.o_head + col;
-            const float v[4] = {acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv};
-            if (a.out_dtype == PSPML_DTYPE_S8) {
-              char4 c;
-              c.x = quantise_s8(v[0], a.out_inv_scale, a.out_zero);
-              c.y = quantise_s8(v[1], a.out_inv_scale, a.out_zero);
-              c.z = quantise_s8(v[2], a.out_inv_scale, a.out_zero);
-              c.w = quantise_s8(v[3], a.out_inv_scale, a.out_zero);
-              *reinterpret_cast<char4*>(static_cast<int8_t*>(a.out) + at) = c;
-            } else {
-              *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + at) =
-                  make_uint2(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]));
+          const int64_t at = orow * a.o_token + oh * a.o_head;
+          constexpr int kCols = 32;
+#pragma unroll 1
+          for (int col = 0; col < DP; col += kCols) {
+            float acc[kCols];
+#pragma unroll
+            for (int y = 0; y < kCols; ++y) acc[y] = 0.0f;
+#pragma unroll 2
+            for (int x = 0; x < p.splits; ++x) {
+              const float2 ml = __ldcg(p.part_ml + (c0 + x) * 256 + tid);
+              const float f = tc_ex2(ml.x - bs);
+              float4 v[kCols / 4];
+#pragma unroll
+              for (int y = 0; y < kCols / 4; ++y)
+                v[y] = __ldcg(p.part_o + ((c0 + x) * (DP / 4) + col / 4 + y) * 256 + tid);
+              if (ml.y != 0.0f)
+#pragma unroll
+                for (int y = 0; y < kCols / 4; ++y) {
+                  acc[4 * y] = fmaf(v[y].x, f, acc[4 * y]);
+                  acc[4 * y + 1] = fmaf(v[y].y, f, acc[4 * y + 1]);
+                  acc[4 * y + 2] = fmaf(v[y].z, f, acc[4 * y + 2]);
+                  acc[4 * y + 3] = fmaf(v[y].w, f, acc[4 * y + 3]);
+                }
             }
+#pragma unroll
+            for (int y = 0; y < kCols; ++y) acc[y] *= inv;
+#pragma unroll
+            for (int y = 0; y < kCols; y += 8)
+              if (col + y < a.dim) store8<T>(a, at + col + y, acc + y);
           }
-          if (col == 0 && a.lse != nullptr)
+          if (a.lse != nullptr)
             a.lse[orow * a.q_heads + oh] =
                 sum == 0.0f ? -INFINITY : (log2f(sum) + bs) * 0.69314718055994531f;
         }
@@ -807,17 +766,19 @@ cudaError_t launch_attn_tc(const AttnArgs& a, const AttnWork& w, cudaStream_t s)
   if (a.paged)
     pairs = std::min(pairs, a.sequences * ((a.max_new + pair_tokens - 1) / pair_tokens));
   const int64_t segments = pairs * a.kv_heads;
-  // Few segments: cut each one's keys so that the parts cover the SMs, with
-  // at least 4 key tiles a part if the sequence is as long as it may be.
+  // Few segments: cut each one's keys into parts, about kPartsPerSm an SM so
+  // that sequences of unlike lengths even out, with at least 4 key tiles a
+  // part if the sequence is as long as it may be.
   const int64_t most_keys = a.paged ? a.pages_stride * a.page_size : a.tokens;
   const int64_t slot = 256 * (dp * static_cast<int64_t>(sizeof(float)) + sizeof(float2));
-  int64_t splits = std::min(w.num_sms / std::max<int64_t>(1, segments), most_keys / (4 * kKeys));
+  int64_t splits = std::min(kPartsPerSm * w.num_sms / std::max<int64_t>(1, segments),
+                            most_keys / (4 * kKeys));
   splits = std::min(splits, static_cast<int64_t>(w.bytes) / std::max<int64_t>(1, segments * slot));
   if (segments > kAttnCounters || splits < 1) splits = 1;
   p.splits = static_cast<int32_t>(splits);
   const int64_t grid = segments * splits;
   if (grid > 0x7FFFFFFF) return cudaErrorInvalidValue;
-  p.part_o = reinterpret_cast<float*>(w.base);
+  p.part_o = reinterpret_cast<float4*>(w.base);
   p.part_ml = reinterpret_cast<float2*>(w.base + grid * 256 * dp * sizeof(float));
 
   CUtensorMap mq, mk, mv;
