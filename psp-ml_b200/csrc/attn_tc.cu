@@ -25,9 +25,12 @@
 // shared memory, since 0 * NaN would spread whatever they hold.  Heads of
 // fewer than DP elements are padded with zeros by TMA.
 //
-// With few tiles the keys of each are cut into equal parts for several CTAs;
-// the unnormalised parts go to the workspace and the CTA that arrives last
-// joins them in order.
+// A CTA stays for many items (a pair of tiles and a key head): the next one's
+// loads and first scores run while this one ends.  Many items are handed out
+// by a counter, those with the most keys first.  Few items are cut: the list
+// of all their key tiles is divided into equal shares, and where a share cuts
+// an item the pieces go to the workspace, unnormalised, and the CTA that
+// arrives last joins them in order, so the same call gives the same bits.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -53,17 +56,27 @@ constexpr int kSoftmaxRegs = 200;
 constexpr int kOtherRegs = 104;
 constexpr int kKeys = 128;        // keys a tile
 constexpr int kPieces = 2;        // in which P is handed to the MMA warp
-constexpr int kPartsPerSm = 2;
+// Calls of fewer items an SM are cut into equal shares.  Cutting costs a piece
+// written and read per cut: six tiles of work an item on 20 heads of 4001
+// tokens take 72 us whole and 104 us cut (2.8 items an SM), 80 items of up to
+// 94 key tiles 189 us whole and 131 us cut.
+constexpr int kItemsPerSm = 2;
+constexpr int kCountedPairs = 64;
 constexpr float kGrowLog2 = 8.0f; // largest stale maximum, as a power of two
 
 struct TcArgs {
   AttnArgs a;
-  float4* part_o;      // [ctas][DP / 4][256]: a warp's rows side by side
-  float2* part_ml;     // [ctas][256]
-  unsigned* arrived;   // [segments]
+  float4* part_o;      // [2 * ctas][DP / 4][256]: a warp's rows side by side
+  float2* part_ml;     // [2 * ctas][256]
+  unsigned* arrived;   // [ctas]
+  unsigned* next;      // first item that no CTA has taken, less the grid's size
+  unsigned* done;      // CTAs that have finished
   unsigned* err;
   float scale_log2;
-  int32_t group, tile_tokens, splits, box_keys;
+  int64_t items;       // pairs * key heads, at most
+  int32_t group, tile_tokens, box_keys;
+  int32_t wide_out;    // output rows start on 32-byte boundaries
+  int32_t shares;      // equal shares of key tiles instead of whole items
 };
 
 template <int DP>
@@ -143,6 +156,23 @@ __device__ __forceinline__ void store8(const AttnArgs& a, int64_t at, const floa
   }
 }
 
+// Sixteen (or, at the end of a head, eight) neighbouring outputs of a row; as
+// one 32-byte sector where the view's alignment allows it.
+template <typename T>
+__device__ __forceinline__ void store16(const AttnArgs& a, int64_t at, const float* v, bool both,
+                                        bool wide) {
+  if (both && wide && a.out_dtype != PSPML_DTYPE_S8) {
+    uint32_t w[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w[i] = pack2<T>(v[2 * i], v[2 * i + 1]);
+    st_global_v8(static_cast<T*>(a.out) + at, make_uint4(w[0], w[1], w[2], w[3]),
+                 make_uint4(w[4], w[5], w[6], w[7]));
+  } else {
+    store8<T>(a, at, v);
+    if (both) store8<T>(a, at + 8, v + 8);
+  }
+}
+
 // Rows, positions and keys of a CTA's two tiles.
 struct TcGeometry {
   int64_t row0;     // first row of the pair in q and out
@@ -154,20 +184,23 @@ struct TcGeometry {
   int tokens0, tokens1;  // of tile A and B
   int tiles0, tiles1;    // key tiles of A and B
 };
+__device__ __forceinline__ unsigned tc_pairs(const TcArgs& p, const SeqSpan& sp) {
+  const int64_t rows = p.a.paged && sp.rows > p.a.max_new ? p.a.max_new : sp.rows;
+  const unsigned pair_tokens = 2u * p.tile_tokens;
+  return (static_cast<unsigned>(rows) + pair_tokens - 1) / pair_tokens;
+}
 // Pair `idx` of the call, found by one warp: the sequences' pairs are counted
 // 32 sequences at a time.  Within a sequence the last tokens come first, so
 // that the pairs with the most keys start first.  False past the last pair.
 __device__ __forceinline__ bool tc_locate(const TcArgs& p, int64_t idx, int lane, int* seq,
                                           int64_t* pair, SeqSpan* span) {
-  const unsigned pair_tokens = 2u * p.tile_tokens;
   for (int s0 = 0; s0 < p.a.sequences; s0 += 32) {
     const int s = s0 + lane;
     SeqSpan sp{0, 0, 0};
     unsigned mine = 0;
     if (s < p.a.sequences) {
       sp = seq_span(p.a, s);
-      const int64_t rows = p.a.paged && sp.rows > p.a.max_new ? p.a.max_new : sp.rows;
-      mine = (static_cast<unsigned>(rows) + pair_tokens - 1) / pair_tokens;
+      mine = tc_pairs(p, sp);
     }
     unsigned scan = mine;
 #pragma unroll
@@ -214,18 +247,45 @@ __device__ __forceinline__ TcGeometry tc_geometry(const TcArgs& p, const SeqSpan
   return g;
 }
 
+// Key tiles that an item counts for: one at least, since its rows have to be
+// written even when they see no key.
+__device__ __forceinline__ int tc_units(const TcGeometry& g) {
+  return max(1, max(g.tiles0, g.tiles1));
+}
+// Key tiles of a sequence for one key head.
+__device__ __forceinline__ int64_t tc_seq_units(const TcArgs& p, const SeqSpan& sp) {
+  int64_t units = 0;
+  const int pairs = static_cast<int>(tc_pairs(p, sp));
+  for (int i = 0; i < pairs; ++i) units += tc_units(tc_geometry(p, sp, i));
+  return units;
+}
+
+// What a CTA's warps need to know of one item, or of its part of one.
+struct TcItem {
+  int64_t row0, place0, keys, lo, start, hi_all;
+  int32_t tokens[2];   // of tile A and B
+  int32_t n[2];        // key tiles of A and B in this part
+  int32_t j0;          // the part's first key tile
+  int32_t head;
+  int32_t pieces;      // CTAs that share the item
+  int32_t first_cta;   // of them
+  int32_t end;         // no more items
+};
+constexpr int kMinShare = 4;     // key tiles of a share, at least
+constexpr uint64_t kItemLimitNs = 5 * kWaitLimitNs;  // longer than any wait within an item
+
 template <typename T, int DP>
 __global__ void __launch_bounds__(kTcThreads, 1)
     k_attn_tc(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
               const __grid_constant__ CUtensorMap map_v, const TcArgs p) {
   using Sh = TcShape<DP>;
   extern __shared__ uint8_t smem_raw[];
-  __shared__ uint64_t q_full, landed, s_full[2], o_done[2], drain;
+  __shared__ uint64_t q_full, q_empty, landed, s_full[2], o_done[2], drain;
   __shared__ uint64_t kv_full[Sh::kSlots], kv_empty[Sh::kSlots];
+  __shared__ uint64_t item_full[2], item_empty[2];
+  __shared__ TcItem items[2];
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_word;
-  __shared__ int64_t s_row0;
-  __shared__ int s_tokens[2];
   __shared__ int s_last;
   const AttnArgs& a = p.a;
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
@@ -234,30 +294,17 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   uint8_t* sq = smem;
   uint8_t* slots = smem + 2 * Sh::kTileBytes;
 
-  const int part = static_cast<int>(blockIdx.x % p.splits);
-  const int64_t seg = blockIdx.x / p.splits;
-  const int head = static_cast<int>(seg % a.kv_heads);
-  int seq;
-  int64_t pair;
-  SeqSpan span;
-  if (!tc_locate(p, seg / a.kv_heads, lane, &seq, &pair, &span)) return;
-  if (warp == 8 && lane == 0) {
-    tma_prefetch_desc(&map_q);
-    tma_prefetch_desc(&map_k);
-    tma_prefetch_desc(&map_v);
-  }
   if (tid == 0) {
-    const TcGeometry g = tc_geometry(p, span, pair);
-    s_row0 = g.row0;
-    s_tokens[0] = g.tokens0;
-    s_tokens[1] = g.tokens1;
     abort_word = 0;
     mbar_init(&q_full, 1);
+    mbar_init(&q_empty, 1);
     mbar_init(&landed, 1);
     mbar_init(&drain, 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s_full[i], 1);
       mbar_init(&o_done[i], 1);
+      mbar_init(&item_full[i], 1);
+      mbar_init(&item_empty[i], 9);  // the MMA warp and eight softmax warps
     }
     for (int i = 0; i < Sh::kSlots; ++i) {
       mbar_init(&kv_full[i], 1);
@@ -266,6 +313,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     fence_mbar_init();
   }
   if (warp == 8) {
+    if (lane == 0) {
+      tma_prefetch_desc(&map_q);
+      tma_prefetch_desc(&map_k);
+      tma_prefetch_desc(&map_v);
+    }
     tmem_alloc(&tmem_slot, Sh::kCols);
     tmem_relinquish();
   }
@@ -273,20 +325,22 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
-
-  const TcGeometry g = tc_geometry(p, span, pair);
-  const int64_t lo = g.lo, start = g.start, hi_all = g.hi_all;
-  const int n_all = max(g.tiles0, g.tiles1);
-  const int j0 = static_cast<int>(static_cast<int64_t>(n_all) * part / p.splits);
-  const int j1 = static_cast<int>(static_cast<int64_t>(n_all) * (part + 1) / p.splits);
-  const int n0 = max(0, min(j1, g.tiles0) - j0), n1 = max(0, min(j1, g.tiles1) - j0);
-  const int n = max(n0, n1);  // key tiles of this CTA
+  // Item `it` of this CTA, published by warp 8.  Whoever has taken an item
+  // walks all of it, and every warp takes the same items: this wait does not
+  // look at the abort flag.
+  auto take = [&](int it) -> const TcItem* {
+    const bool got =
+        __all_sync(~0u, mbar_wait(&item_full[it & 1], static_cast<uint32_t>((it >> 1) & 1),
+                                  nullptr, kItemLimitNs));
+    if (!got && lane == 0) tc_fail(p.err, abort, kDevErrEpiWait);
+    return got ? &items[it & 1] : nullptr;
+  };
   // Keys of tile j that some row sees: [v_lo, v_hi) of its 128.
-  auto v_lo = [&](int j) {
+  auto v_lo = [](int64_t lo, int64_t start, int j) {
     const int64_t x = lo - (start + static_cast<int64_t>(j) * kKeys);
     return x > 0 ? static_cast<int>(x) : 0;
   };
-  auto v_hi = [&](int j) {
+  auto v_hi = [](int64_t hi_all, int64_t start, int j) {
     const int64_t x = hi_all - (start + static_cast<int64_t>(j) * kKeys);
     return x < kKeys ? static_cast<int>(x) : kKeys;
   };
@@ -294,101 +348,241 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
   if (warp == 8) {
-    // ---------------------------------------------------------- TMA loads
+    // ------------------------------------------------- items and TMA loads
     const int boxes = kKeys / p.box_keys;  // one per lane
-    const int32_t* table = a.paged ? a.pages + seq * a.pages_stride : nullptr;
-    auto page_of = [&](int j) -> int {
-      const int64_t key = start + static_cast<int64_t>(j) * kKeys + lane * p.box_keys;
-      if (!a.paged || lane >= boxes || key < 0 || key + p.box_keys <= lo || key >= hi_all) return -1;
-      return table[key / a.page_size];
-    };
-    if (n > 0 && lane == 0) {
-      const int active = (n0 > 0) + (n1 > 0);
-      mbar_arrive_expect_tx(
-          &q_full, static_cast<uint32_t>(active * Sh::kHalves * p.tile_tokens * p.group * 128));
-      for (int t = 0; t < 2; ++t) {
-        if ((t == 0 ? n0 : n1) == 0) continue;
-        for (int h = 0; h < Sh::kHalves; ++h)
-          tma_load_4d(sq + t * Sh::kTileBytes + h * 16384, &map_q, &q_full, h * 128, 0, head,
-                      static_cast<int32_t>(g.row0 + t * p.tile_tokens));
+    int slot = 0, landings = 0, issued = 0, q_loads = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    int64_t next = blockIdx.x;  // handed out: the item
+    int seq = 0, head = 0, tile = 0;
+    int64_t pair = 0;
+    SeqSpan span{0, 0, 0};
+    int64_t total = 0, at = 0, stop = 0, ctas = 0;  // shares: key tiles, this CTA's, CTAs in use
+    if (p.shares) {
+      for (int s0 = 0; s0 < a.sequences; s0 += 32) {
+        int64_t u = s0 + lane < a.sequences ? tc_seq_units(p, seq_span(a, s0 + lane)) : 0;
+#pragma unroll
+        for (int o = 16; o > 0; o /= 2) u += __shfl_xor_sync(~0u, u, o);
+        total += u * a.kv_heads;
+      }
+      const int64_t wanted = (total + kMinShare - 1) / kMinShare;
+      ctas = wanted < gridDim.x ? wanted : gridDim.x;
+      if (blockIdx.x < ctas) {
+        at = blockIdx.x * total / ctas;
+        stop = (blockIdx.x + 1) * total / ctas;
+        // The sequence, pair, head and tile that the share begins with.
+        int64_t before = 0;
+        for (int s0 = 0;; s0 += 32) {
+          SeqSpan sp{0, 0, 0};
+          if (s0 + lane < a.sequences) sp = seq_span(a, s0 + lane);
+          int64_t scan = tc_seq_units(p, sp) * a.kv_heads;
+#pragma unroll
+          for (int o = 1; o < 32; o *= 2) {
+            const int64_t v = __shfl_up_sync(~0u, scan, o);
+            if (lane >= o) scan += v;
+          }
+          const unsigned past = __ballot_sync(~0u, at < before + scan);
+          if (past != 0) {
+            const int who = __ffs(past) - 1;
+            seq = s0 + who;
+            span.begin = __shfl_sync(~0u, sp.begin, who);
+            span.keys = __shfl_sync(~0u, sp.keys, who);
+            span.rows = __shfl_sync(~0u, sp.rows, who);
+            if (who > 0) before += __shfl_sync(~0u, scan, who - 1);
+            break;
+          }
+          before += __shfl_sync(~0u, scan, 31);
+        }
+        pair = static_cast<int64_t>(tc_pairs(p, span)) - 1;
+        while (true) {
+          const int u = tc_units(tc_geometry(p, span, pair));
+          if (at < before + static_cast<int64_t>(u) * a.kv_heads) {
+            head = static_cast<int>((at - before) / u);
+            tile = static_cast<int>((at - before) - static_cast<int64_t>(head) * u);
+            break;
+          }
+          before += static_cast<int64_t>(u) * a.kv_heads;
+          --pair;
+        }
       }
     }
-    int slot = 0, landings = 0;
-    uint32_t phase = 0;
-    int issued = 0;
-    bool ok = true;
-    int page = n > 0 ? page_of(j0) : -1;
-    for (int j = j0; j < j0 + n && ok; ++j) {
-      const int64_t kb = start + static_cast<int64_t>(j) * kKeys;
-      const int lo_k = v_lo(j), hi_k = v_hi(j);
-      const int first = lane * p.box_keys;
-      const bool load = lane < boxes && first < hi_k && first + p.box_keys > lo_k;
-      const int n_load = __popc(__ballot_sync(~0u, load));
-      const uint32_t bytes = static_cast<uint32_t>(n_load * p.box_keys * 128 * Sh::kHalves);
-      const int next_page = j + 1 < j0 + n ? page_of(j + 1) : -1;
-      const int32_t c2 = a.paged ? static_cast<int32_t>((kb + first) % a.page_size)
-                                 : static_cast<int32_t>(g.row0 - g.place0 + kb + first);
-      const int32_t c3 = a.paged ? page : 0;
-      for (int which = 0; which < 2; ++which) {
-        if (!mbar_wait(&kv_empty[slot], phase ^ 1u, abort)) {
+    for (int it = 0;; ++it) {
+      TcItem* const d = &items[it & 1];
+      if (it >= 2 && !mbar_wait(&item_empty[it & 1], static_cast<uint32_t>(((it >> 1) - 1) & 1),
+                                nullptr, kItemLimitNs)) {
+        tc_fail(p.err, abort, kDevErrTmaWait);
+        ok = false;
+      }
+      bool have = __all_sync(~0u, ok && !*abort);
+      if (p.shares) {
+        have = have && at < stop;
+      } else {
+        head = static_cast<int>(next % a.kv_heads);
+        have = have && next < p.items &&
+               tc_locate(p, next / a.kv_heads, lane, &seq, &pair, &span);
+      }
+      if (!have) {
+        if (lane == 0) {
+          d->end = 1;
+          mbar_arrive(&item_full[it & 1]);
+        }
+        break;
+      }
+      const TcGeometry g = tc_geometry(p, span, pair);
+      const int64_t lo = g.lo, start = g.start, hi_all = g.hi_all;
+      const int units = tc_units(g), j0 = tile;
+      int j1 = units, pieces = 1, first_cta = 0;
+      if (p.shares) {
+        if (stop - at < j1 - j0) j1 = j0 + static_cast<int>(stop - at);
+        if (j0 > 0 || j1 < units) {
+          // Tile f of the list belongs to CTA ((f + 1) * ctas - 1) / total.
+          const int64_t f = at - j0;
+          first_cta = static_cast<int>(((f + 1) * ctas - 1) / total);
+          pieces = static_cast<int>(((f + units) * ctas - 1) / total) - first_cta + 1;
+        }
+      }
+      const int n0 = max(0, min(j1, g.tiles0) - j0), n1 = max(0, min(j1, g.tiles1) - j0);
+      const int n = max(n0, n1);
+      if (lane == 0) {
+        d->row0 = g.row0;
+        d->place0 = g.place0;
+        d->keys = g.keys;
+        d->lo = lo;
+        d->start = start;
+        d->hi_all = hi_all;
+        d->tokens[0] = g.tokens0;
+        d->tokens[1] = g.tokens1;
+        d->n[0] = n0;
+        d->n[1] = n1;
+        d->j0 = j0;
+        d->head = head;
+        d->pieces = pieces;
+        d->first_cta = first_cta;
+        d->end = 0;
+        mbar_arrive(&item_full[it & 1]);
+      }
+      __syncwarp();
+      // The next item: asked for now, looked at when this one's loads are out.
+      unsigned taken = 0;
+      const bool more = !p.shares && p.items > gridDim.x;
+      if (more && lane == 0) taken = atomicAdd(p.next, 1u);
+
+      const int32_t* table = a.paged ? a.pages + seq * a.pages_stride : nullptr;
+      auto page_of = [&](int j) -> int {
+        const int64_t key = start + static_cast<int64_t>(j) * kKeys + lane * p.box_keys;
+        if (!a.paged || lane >= boxes || key + p.box_keys <= lo || key >= hi_all) return -1;
+        return table[static_cast<uint32_t>(key) / static_cast<uint32_t>(a.page_size)];
+      };
+      int page = n > 0 ? page_of(j0) : -1;
+      if (n > 0) {
+        if (q_loads > 0 && !mbar_wait(&q_empty, static_cast<uint32_t>((q_loads - 1) & 1), abort)) {
           tc_fail(p.err, abort, kDevErrTmaWait);
           ok = false;
-          break;
         }
-        uint8_t* dst = slots + slot * Sh::kTileBytes;
-        const bool mend = which == 1 && ((lo_k | hi_k) & 15) != 0;
-        uint64_t* bar = mend ? &landed : &kv_full[slot];
-        if (lane == 0) mbar_arrive_expect_tx(bar, bytes);
         __syncwarp();
-        if (load)
-          for (int h = 0; h < Sh::kHalves; ++h)
-            tma_load_4d(dst + h * 16384 + first * 128, which ? &map_v : &map_k, bar, h * 128, head,
-                        c2, c3);
-        __syncwarp();
-        if (mend) {
-          if (!mbar_wait(&landed, static_cast<uint32_t>(landings & 1), abort)) {
-            tc_fail(p.err, abort, kDevErrTmaWait);
-            ok = false;
+        if (lane == 0) {
+          const int active = (n0 > 0) + (n1 > 0);
+          mbar_arrive_expect_tx(
+              &q_full, static_cast<uint32_t>(active * Sh::kHalves * p.tile_tokens * p.group * 128));
+          for (int t = 0; t < 2; ++t) {
+            if ((t == 0 ? n0 : n1) == 0) continue;
+            for (int h = 0; h < Sh::kHalves; ++h)
+              tma_load_4d(sq + t * Sh::kTileBytes + h * 16384, &map_q, &q_full, h * 128, 0, head,
+                          static_cast<int32_t>(g.row0 + t * p.tile_tokens));
           }
-          ++landings;
-          const int a0 = lo_k & ~15, a1 = (hi_k + 15) & ~15;
-          const int dead = (lo_k - a0) + (a1 - hi_k);
-          for (int u = lane; u < dead * 8 * Sh::kHalves; u += 32) {
-            const int i = u / (8 * Sh::kHalves), c = u % (8 * Sh::kHalves);
-            const int r = i < lo_k - a0 ? a0 + i : hi_k + (i - (lo_k - a0));
-            *reinterpret_cast<uint4*>(dst + (c / 8) * 16384 + r * 128 + (c % 8) * 16) =
-                make_uint4(0, 0, 0, 0);
-          }
-          fence_async_smem();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&kv_full[slot]);
         }
-        ++issued;
-        if (++slot == Sh::kSlots) {
-          slot = 0;
-          phase ^= 1u;
-        }
+        ++q_loads;
       }
-      page = next_page;
+      for (int j = j0; j < j0 + n && ok; ++j) {
+        const int64_t kb = start + static_cast<int64_t>(j) * kKeys;
+        const int lo_k = v_lo(lo, start, j), hi_k = v_hi(hi_all, start, j);
+        const int first = lane * p.box_keys;
+        const bool load = lane < boxes && first < hi_k && first + p.box_keys > lo_k;
+        const int n_load = __popc(__ballot_sync(~0u, load));
+        const uint32_t bytes = static_cast<uint32_t>(n_load * p.box_keys * 128 * Sh::kHalves);
+        const int next_page = j + 1 < j0 + n ? page_of(j + 1) : -1;
+        const int32_t c2 = a.paged ? static_cast<int32_t>(static_cast<uint32_t>(kb + first) %
+                                                          static_cast<uint32_t>(a.page_size))
+                                   : static_cast<int32_t>(span.begin + kb + first);
+        const int32_t c3 = a.paged ? page : 0;
+        for (int which = 0; which < 2; ++which) {
+          const bool got = mbar_wait(&kv_empty[slot], phase ^ 1u, abort);
+          if (!got) tc_fail(p.err, abort, kDevErrTmaWait);
+          if (!__all_sync(~0u, got)) {
+            ok = false;
+            break;
+          }
+          uint8_t* dst = slots + slot * Sh::kTileBytes;
+          const bool mend = which == 1 && ((lo_k | hi_k) & 15) != 0;
+          uint64_t* bar = mend ? &landed : &kv_full[slot];
+          if (lane == 0) mbar_arrive_expect_tx(bar, bytes);
+          __syncwarp();
+          if (load)
+            for (int h = 0; h < Sh::kHalves; ++h)
+              tma_load_4d(dst + h * 16384 + first * 128, which ? &map_v : &map_k, bar, h * 128,
+                          head, c2, c3);
+          __syncwarp();
+          if (mend) {
+            if (!mbar_wait(&landed, static_cast<uint32_t>(landings & 1), abort)) {
+              tc_fail(p.err, abort, kDevErrTmaWait);
+              ok = false;
+            }
+            ++landings;
+            const int a0 = lo_k & ~15, a1 = (hi_k + 15) & ~15;
+            const int dead = (lo_k - a0) + (a1 - hi_k);
+            for (int u = lane; u < dead * 8 * Sh::kHalves; u += 32) {
+              const int i = u / (8 * Sh::kHalves), c = u % (8 * Sh::kHalves);
+              const int r = i < lo_k - a0 ? a0 + i : hi_k + (i - (lo_k - a0));
+              *reinterpret_cast<uint4*>(dst + (c / 8) * 16384 + r * 128 + (c % 8) * 16) =
+                  make_uint4(0, 0, 0, 0);
+            }
+            fence_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&kv_full[slot]);
+          }
+          ++issued;
+          if (++slot == Sh::kSlots) {
+            slot = 0;
+            phase ^= 1u;
+          }
+        }
+        ok = __all_sync(~0u, ok);
+        page = next_page;
+      }
+      if (!p.shares) {
+        next = more ? static_cast<int64_t>(__shfl_sync(~0u, taken, 0)) + gridDim.x : p.items;
+        continue;
+      }
+      at += j1 - j0;
+      tile = j1 < units ? j1 : 0;
+      if (tile == 0 && ++head == a.kv_heads) {
+        head = 0;
+        if (--pair < 0)
+          while (++seq < a.sequences) {
+            span = seq_span(a, seq);
+            pair = static_cast<int64_t>(tc_pairs(p, span)) - 1;
+            if (pair >= 0) break;
+          }
+      }
     }
-    if (*abort) {  // the copies in flight land before the CTA leaves
-      if (n > 0) mbar_wait(&q_full, 0, nullptr);
+    if (__any_sync(~0u, *abort)) {  // the copies in flight land before the CTA leaves
+      if (q_loads > 0) mbar_wait(&q_full, static_cast<uint32_t>((q_loads - 1) & 1), nullptr);
+      if (landings > 0) mbar_wait(&landed, static_cast<uint32_t>((landings - 1) & 1), nullptr);
       for (int i = issued > Sh::kSlots ? issued - Sh::kSlots : 0; i < issued; ++i)
         mbar_wait(&kv_full[i % Sh::kSlots], static_cast<uint32_t>((i / Sh::kSlots) & 1), nullptr);
     }
+    __syncwarp();
   } else if (warp == 9) {
     // --------------------------------------------------------------- MMAs
     // The whole warp walks the loop and its waits; elect.sync names the one
     // lane that issues, which is how the compiler knows that the operands of
     // an MMA are one thread's and moves them to the tensor core directly.
-    if (n > 0) {
+    {
       constexpr int kFmt = std::is_same<T, __half>::value ? 0 : 1;
       const int k_steps = (a.dim + 15) / 16;
       const uint32_t id_qk = make_idesc_f16(128, kKeys, kFmt, 0);
       const uint32_t id_pv = make_idesc_f16(128, k_steps * 16, kFmt, 1);
       const uint32_t q_addr = smem_u32(sq), kv_addr = smem_u32(slots);
-      const int k_first = v_lo(j0) / 16;                  // steps of the first key tile
-      const int k_last = (v_hi(j0 + n - 1) + 15) / 16;    // and of the last
       // A wait that gives up only raises the abort flag, after which every
       // other wait ends at once.
       auto wait = [&](uint64_t* bar, uint32_t phase) {
@@ -416,8 +610,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       };
       // P comes in pieces: the product of one runs while the next one's
       // weights are found.
-      auto pv = [&](int t, int i, int slot, uint64_t* freed) {
-        const int k0 = i == 0 ? k_first : 0, k1 = i == n - 1 ? k_last : kKeys / 16;
+      auto pv = [&](int t, int i, int slot, int k0, int k1, uint64_t* freed) {
 #pragma unroll
         for (int h = 0; h < kPieces; ++h) {
           prob_wait(t, h);
@@ -437,35 +630,66 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           __syncwarp();
         }
       };
-      wait(&q_full, 0);
-      wait(&kv_full[0], 0);
-      if (n0 > 0) qk(0, 0, n1 > 0 ? nullptr : &kv_empty[0]);
-      if (n1 > 0) qk(1, 0, &kv_empty[0]);
-      int v_slot = 1, k_slot = 2;  // ring slots of value tile i and key tile i + 1
-      uint32_t v_phase = 0, k_phase = 0;
-      for (int i = 0; i < n; ++i) {
-        wait(&kv_full[v_slot], v_phase);
-        if (i + 1 < n) wait(&kv_full[k_slot], k_phase);
+      uint32_t done[2] = {0, 0};   // key tiles of A and of B so far
+      int k_slot = 0, q_items = 0; // ring slot and phase of the next key tile
+      uint32_t k_phase = 0;
+      for (int it = 0;; ++it) {
+        const TcItem* const d = take(it);
+        if (d == nullptr || d->end) break;
+        const int n0 = d->n[0], n1 = d->n[1], n = max(n0, n1);
+        if (n > 0) {
+          const int k_first = v_lo(d->lo, d->start, d->j0) / 16;  // steps of the first key tile
+          const int k_last = (v_hi(d->hi_all, d->start, d->j0 + n - 1) + 15) / 16;  // of the last
+          wait(&q_full, static_cast<uint32_t>(q_items & 1));
+          ++q_items;
+          wait(&kv_full[k_slot], k_phase);
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          const int nt = t == 0 ? n0 : n1, other = t == 0 ? n1 : 0;
-          if (i >= nt) continue;
-          pv(t, i, v_slot, i < other ? nullptr : &kv_empty[v_slot]);
-          if (i + 1 >= nt) continue;
-          // P is read before the next S is written over it.
-          wait(&o_done[t], static_cast<uint32_t>(i & 1));
-          qk(t, k_slot, i + 1 < other ? nullptr : &kv_empty[k_slot]);
+          for (int t = 0; t < 2; ++t) {
+            const int nt = t == 0 ? n0 : n1;
+            if (nt == 0) continue;
+            if (done[t] > 0) wait(&o_done[t], (done[t] - 1) & 1u);
+            qk(t, k_slot, t == 0 && n1 > 0 ? nullptr : &kv_empty[k_slot]);
+          }
+          if (n == 1) {
+            if (elect_one()) umma_commit(&q_empty);
+            __syncwarp();
+          }
+          for (int i = 0; i < n; ++i) {
+            int v_slot = k_slot + 1;
+            uint32_t v_phase = k_phase;
+            if (v_slot == Sh::kSlots) {
+              v_slot = 0;
+              v_phase ^= 1u;
+            }
+            k_slot = v_slot + 1;
+            k_phase = v_phase;
+            if (k_slot == Sh::kSlots) {
+              k_slot = 0;
+              k_phase ^= 1u;
+            }
+            wait(&kv_full[v_slot], v_phase);
+            if (i + 1 < n) wait(&kv_full[k_slot], k_phase);
+            const int k0 = i == 0 ? k_first : 0, k1 = i == n - 1 ? k_last : kKeys / 16;
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+              const int nt = t == 0 ? n0 : n1, other = t == 0 ? n1 : 0;
+              if (i >= nt) continue;
+              pv(t, i, v_slot, k0, k1, i < other ? nullptr : &kv_empty[v_slot]);
+              if (i + 1 >= nt) continue;
+              // P is read before the next S is written over it.
+              wait(&o_done[t], (done[t] + static_cast<uint32_t>(i)) & 1u);
+              qk(t, k_slot, i + 1 < other ? nullptr : &kv_empty[k_slot]);
+            }
+            if (i + 2 == n) {  // the item's last scores are on their way: Q may be replaced
+              if (elect_one()) umma_commit(&q_empty);
+              __syncwarp();
+            }
+          }
+          done[0] += static_cast<uint32_t>(n0);
+          done[1] += static_cast<uint32_t>(n1);
         }
-        v_slot += 2;
-        if (v_slot >= Sh::kSlots) {
-          v_slot -= Sh::kSlots;
-          v_phase ^= 1u;
-        }
-        k_slot += 2;
-        if (k_slot >= Sh::kSlots) {
-          k_slot -= Sh::kSlots;
-          k_phase ^= 1u;
-        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&item_empty[it & 1]);
       }
       // Every MMA completes before tensor memory is freed.
       if (elect_one()) umma_commit(&drain);
@@ -478,30 +702,39 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
     // ------------------------------------------------------------ softmax
     const int t = warp / 4;
-    const int nt = t == 0 ? n0 : n1;
     const int row = tid % 128;
-    // The row's keys [row_beg, row_end), and those that every row of the tile
-    // sees, counted from the first key tile.
-    const int64_t place = g.place0 + t * p.tile_tokens;  // of the tile's first token
-    const int tok = row / p.group;
-    auto end_of = [&](int64_t at) {
-      const int64_t e = a.causal && at + 1 < g.keys ? at + 1 : g.keys;
-      return static_cast<int>(e > start ? e - start : 0);
-    };
-    auto beg_of = [&](int64_t at) {
-      const int64_t b = a.window > 0 ? at - a.window + 1 : 0;
-      return static_cast<int>(b > start ? b - start : 0);
-    };
-    const int row_end = end_of(place + tok), row_beg = beg_of(place + tok);
-    const int all_end = end_of(place);
-    const int all_beg = beg_of(place + (t == 0 ? g.tokens0 : g.tokens1) - 1);
     const uint32_t lanes = static_cast<uint32_t>((warp % 4) * 32) << 16;
     const uint32_t ts = tmem + Sh::kS + t * 128 + lanes, to = tmem + Sh::kO + t * DP + lanes;
+    uint32_t done = 0;  // key tiles so far
+    for (int it = 0;; ++it) {
+    const TcItem* const d = take(it);
+    if (d == nullptr || d->end) break;
+    const int nt = d->n[t];
+    // The row's keys [row_beg, row_end), and those that every row of the tile
+    // sees, counted from the part's first key tile.
+    int row_beg, row_end, all_beg, all_end;
+    {
+      const int64_t first = d->start + static_cast<int64_t>(d->j0) * kKeys;
+      const int64_t place = d->place0 + t * p.tile_tokens;  // of the tile's first token
+      auto end_of = [&](int64_t at) {
+        const int64_t e = a.causal && at + 1 < d->keys ? at + 1 : d->keys;
+        return static_cast<int>(e > first ? e - first : 0);
+      };
+      auto beg_of = [&](int64_t at) {
+        const int64_t b = a.window > 0 ? at - a.window + 1 : 0;
+        return static_cast<int>(b > first ? b - first : 0);
+      };
+      const int tok = row / p.group;
+      row_end = end_of(place + tok);
+      row_beg = beg_of(place + tok);
+      all_end = end_of(place);
+      all_beg = beg_of(place + d->tokens[t] - 1);
+    }
     float m = -INFINITY, l = 0.0f;
     bool ok = true;
     for (int i = 0; i < nt; ++i) {
-      const int kb = (j0 + i) * kKeys;
-      if (!mbar_wait(&s_full[t], static_cast<uint32_t>(i & 1), abort)) {
+      const int kb = i * kKeys;
+      if (!mbar_wait(&s_full[t], (done + static_cast<uint32_t>(i)) & 1u, abort)) {
         tc_fail(p.err, abort, kDevErrEpiWait);
         ok = false;
       }
@@ -570,22 +803,26 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       f2_get(sums[1], sc, sd);
       l += (sa + sb) + (sc + sd);
     }
+    done += static_cast<uint32_t>(nt);
     if (nt > 0 && ok) {
-      ok = mbar_wait(&o_done[t], static_cast<uint32_t>((nt - 1) & 1), abort);
+      ok = mbar_wait(&o_done[t], (done - 1) & 1u, abort);
       if (!ok) tc_fail(p.err, abort, kDevErrEpiWait);
       __syncwarp();
       tc_fence_after();
     }
     ok = __all_sync(~0u, ok);
     // Read back here so that the loop above does not carry them in registers.
-    const int64_t row0 = *const_cast<volatile int64_t*>(&s_row0);
+    const volatile TcItem* const v_item = &items[it & 1];
+    const int64_t row0 = v_item->row0;
+    const int head = v_item->head, pieces = v_item->pieces, first_cta = v_item->first_cta;
+    // This CTA's piece: it ends the CTA's share if the item begins here.
+    const int64_t slot = 2 * static_cast<int64_t>(blockIdx.x) + (v_item->j0 == 0 ? 1 : 0);
     const int tk = row / p.group;
-    const bool real = tk < *const_cast<volatile int*>(&s_tokens[t]);
+    const bool real = tk < v_item->tokens[t];
     const int64_t out_row = row0 + t * p.tile_tokens + tk;
     const int h = head * p.group + (row - tk * p.group);
-    const int64_t cta = static_cast<int64_t>(blockIdx.x);
     if (ok) {
-      const float f = p.splits > 1 ? 1.0f : (l == 0.0f ? 0.0f : 1.0f / l);
+      const float f = pieces > 1 ? 1.0f : (l == 0.0f ? 0.0f : 1.0f / l);
       const int64_t at = out_row * a.o_token + h * a.o_head;
 #pragma unroll 1
       for (int c = 0; c < DP / 32; ++c) {
@@ -600,12 +837,13 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 #pragma unroll
         for (int x = 0; x < 32; ++x) v[x] = __uint_as_float(o[x]) * f;
         if (real) {
-          if (p.splits == 1) {
+          if (pieces == 1) {
 #pragma unroll
-            for (int x = 0; x < 32; x += 8)
-              if (c * 32 + x < a.dim) store8<T>(a, at + c * 32 + x, v + x);
+            for (int x = 0; x < 32; x += 16)
+              if (c * 32 + x < a.dim)
+                store16<T>(a, at + c * 32 + x, v + x, c * 32 + x + 16 <= a.dim, p.wide_out);
           } else {
-            float4* dst = p.part_o + (cta * (DP / 4) + c * 8) * 256 + t * 128 + row;
+            float4* dst = p.part_o + (slot * (DP / 4) + c * 8) * 256 + t * 128 + row;
 #pragma unroll
             for (int x = 0; x < 8; ++x)
               dst[x * 256] = make_float4(v[4 * x], v[4 * x + 1], v[4 * x + 2], v[4 * x + 3]);
@@ -613,33 +851,35 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         }
       }
       const float ml = m == -INFINITY ? -INFINITY : m * p.scale_log2;
-      if (real && p.splits > 1) p.part_ml[cta * 256 + t * 128 + row] = make_float2(ml, l);
-      if (real && p.splits == 1 && a.lse != nullptr)
+      if (real && pieces > 1) p.part_ml[slot * 256 + t * 128 + row] = make_float2(ml, l);
+      if (real && pieces == 1 && a.lse != nullptr)
         a.lse[out_row * a.q_heads + h] =
             l == 0.0f ? -INFINITY : (log2f(l) + ml) * 0.69314718055994531f;
     }
-    if (p.splits > 1) {
+    if (pieces > 1) {
       __threadfence();
       asm volatile("bar.sync 1, 256;" ::: "memory");
       if (tid == 0) {
-        const unsigned arrived = atomicAdd(p.arrived + seg, 1u);
-        s_last = arrived + 1 == static_cast<unsigned>(p.splits);
-        if (s_last) p.arrived[seg] = 0;
+        const unsigned arrived = atomicAdd(p.arrived + first_cta, 1u);
+        s_last = arrived + 1 == static_cast<unsigned>(pieces);
+        if (s_last) p.arrived[first_cta] = 0;
       }
       asm volatile("bar.sync 1, 256;" ::: "memory");
       if (s_last) {
         __threadfence();
-        // Each thread joins a row: its maximum and sum over the parts, then
-        // its columns, kCols at a time.  A part without a key that counts
+        // Each thread joins a row: its maximum and sum over the pieces, then
+        // its columns, kCols at a time.  A piece without a key that counts
         // (sum 0) has nothing to add.
-        const int64_t c0 = cta - part;
+        auto slot_of = [&](int x) {
+          return 2 * static_cast<int64_t>(first_cta + x) + (x == 0 ? 1 : 0);
+        };
         const int tt = tid / 128, rr = tid % 128;
         const int jt = rr / p.group;
-        if (jt < s_tokens[tt]) {
+        if (jt < v_item->tokens[tt]) {
           float mm = -INFINITY, sum = 0.0f;
 #pragma unroll 4
-          for (int x = 0; x < p.splits; ++x) {
-            const float2 ml = __ldcg(p.part_ml + (c0 + x) * 256 + tid);
+          for (int x = 0; x < pieces; ++x) {
+            const float2 ml = __ldcg(p.part_ml + slot_of(x) * 256 + tid);
             const float top = fmaxf(mm, ml.x);
             const float bs = top == -INFINITY ? 0.0f : top;
             sum = sum * tc_ex2(mm - bs) + ml.y * tc_ex2(ml.x - bs);
@@ -657,13 +897,13 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 #pragma unroll
             for (int y = 0; y < kCols; ++y) acc[y] = 0.0f;
 #pragma unroll 2
-            for (int x = 0; x < p.splits; ++x) {
-              const float2 ml = __ldcg(p.part_ml + (c0 + x) * 256 + tid);
+            for (int x = 0; x < pieces; ++x) {
+              const float2 ml = __ldcg(p.part_ml + slot_of(x) * 256 + tid);
               const float f = tc_ex2(ml.x - bs);
               float4 v[kCols / 4];
 #pragma unroll
               for (int y = 0; y < kCols / 4; ++y)
-                v[y] = __ldcg(p.part_o + ((c0 + x) * (DP / 4) + col / 4 + y) * 256 + tid);
+                v[y] = __ldcg(p.part_o + (slot_of(x) * (DP / 4) + col / 4 + y) * 256 + tid);
               if (ml.y != 0.0f)
 #pragma unroll
                 for (int y = 0; y < kCols / 4; ++y) {
@@ -676,8 +916,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 #pragma unroll
             for (int y = 0; y < kCols; ++y) acc[y] *= inv;
 #pragma unroll
-            for (int y = 0; y < kCols; y += 8)
-              if (col + y < a.dim) store8<T>(a, at + col + y, acc + y);
+            for (int y = 0; y < kCols; y += 16)
+              if (col + y < a.dim)
+                store16<T>(a, at + col + y, acc + y, col + y + 16 <= a.dim, p.wide_out);
           }
           if (a.lse != nullptr)
             a.lse[orow * a.q_heads + oh] =
@@ -685,12 +926,21 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         }
       }
     }
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&item_empty[it & 1]);
+    }
     tc_fence_before();
   }
   __syncthreads();
   if (warp == 8) {
     tc_fence_after();
     tmem_dealloc(tmem, Sh::kCols);
+  }
+  // Every CTA has asked for its last item: the last one out leaves the
+  // counters as it found them.
+  if (tid == 0 && !p.shares && p.items > gridDim.x && atomicAdd(p.done, 1u) + 1 == gridDim.x) {
+    *p.next = 0;
+    *p.done = 0;
   }
 }
 
@@ -758,6 +1008,7 @@ cudaError_t launch_attn_tc(const AttnArgs& a, const AttnWork& w, cudaStream_t s)
   p.scale_log2 = a.scale * 1.4426950408889634f;
   p.group = a.q_heads / a.kv_heads;
   p.tile_tokens = 128 / p.group;
+  p.wide_out = reinterpret_cast<uintptr_t>(a.out) % 32 == 0 && (a.o_token | a.o_head) % 16 == 0;
   p.box_keys = a.paged ? pow2_gcd128(a.page_size) : kKeys;
 
   // Pairs at most: every sequence may end in a part of one.
@@ -765,21 +1016,28 @@ cudaError_t launch_attn_tc(const AttnArgs& a, const AttnWork& w, cudaStream_t s)
   int64_t pairs = a.tokens / pair_tokens + a.sequences;
   if (a.paged)
     pairs = std::min(pairs, a.sequences * ((a.max_new + pair_tokens - 1) / pair_tokens));
-  const int64_t segments = pairs * a.kv_heads;
-  // Few segments: cut each one's keys into parts, about kPartsPerSm an SM so
-  // that sequences of unlike lengths even out, with at least 4 key tiles a
-  // part if the sequence is as long as it may be.
-  const int64_t most_keys = a.paged ? a.pages_stride * a.page_size : a.tokens;
+  p.items = pairs * a.kv_heads;
+  if (p.items > 0x7FFFFFFF) return cudaErrorInvalidValue;
+  // Fewer than kItemsPerSm items an SM leave some SMs idle at the end: equal
+  // shares then, as long as a warp can count a sequence's key tiles quickly.
   const int64_t slot = 256 * (dp * static_cast<int64_t>(sizeof(float)) + sizeof(float2));
-  int64_t splits = std::min(kPartsPerSm * w.num_sms / std::max<int64_t>(1, segments),
-                            most_keys / (4 * kKeys));
-  splits = std::min(splits, static_cast<int64_t>(w.bytes) / std::max<int64_t>(1, segments * slot));
-  if (segments > kAttnCounters || splits < 1) splits = 1;
-  p.splits = static_cast<int32_t>(splits);
-  const int64_t grid = segments * splits;
-  if (grid > 0x7FFFFFFF) return cudaErrorInvalidValue;
+  const int64_t seq_tokens = a.paged ? std::min<int64_t>(a.tokens, a.max_new) : a.tokens;
+  const int64_t most_keys = a.paged ? a.pages_stride * a.page_size : a.tokens;
+  int64_t grid = std::min<int64_t>(w.num_sms, kAttnCounters - 2);
+  p.shares = p.items < static_cast<int64_t>(kItemsPerSm) * grid &&
+             seq_tokens / pair_tokens < kCountedPairs && 2 * slot <= static_cast<int64_t>(w.bytes) &&
+             most_keys > kMinShare * kKeys;
+  if (p.shares) {
+    grid = std::min(grid, static_cast<int64_t>(w.bytes) / (2 * slot));
+    grid = std::min(grid, p.items * ((most_keys + kMinShare * kKeys - 1) / (kMinShare * kKeys)));
+    grid = std::max<int64_t>(grid, 1);
+  } else {
+    grid = std::min(grid, p.items);
+  }
+  p.next = w.counters + kAttnCounters - 2;
+  p.done = w.counters + kAttnCounters - 1;
   p.part_o = reinterpret_cast<float4*>(w.base);
-  p.part_ml = reinterpret_cast<float2*>(w.base + grid * 256 * dp * sizeof(float));
+  p.part_ml = reinterpret_cast<float2*>(w.base + 2 * grid * 256 * dp * sizeof(float));
 
   CUtensorMap mq, mk, mv;
   const uint64_t dim = a.dim, hkv = a.kv_heads, tok = a.tokens;
