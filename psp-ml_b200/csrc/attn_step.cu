@@ -44,7 +44,6 @@ struct StepArgs {
   unsigned* arrived;   // [ctas], zero between calls
   float scale_log2;
   int32_t group;
-  int32_t min_tiles;
 };
 
 template <int DP>
@@ -148,6 +147,14 @@ __device__ __forceinline__ void step_advance(const StepArgs& p, StepCursor& c) {
   step_next_seq(p, c);
 }
 
+// First tile of CTA c's share; in 32 bits, a fraction of the time, when the
+// product fits.
+__device__ __forceinline__ int64_t share_of(unsigned c, int64_t total, int64_t ctas) {
+  if (total < (1 << 21))  // at most 1024 CTAs
+    return c * static_cast<uint32_t>(total) / static_cast<uint32_t>(ctas);
+  return static_cast<int64_t>(c) * total / ctas;
+}
+
 // Writes a row pair's two neighbouring outputs.
 template <typename T>
 __device__ __forceinline__ void store2(const AttnArgs& a, int64_t at, float x, float y) {
@@ -168,18 +175,24 @@ __global__ void __launch_bounds__(kStepThreads, kStepCtasPerSm) k_attn_step(cons
   __shared__ int64_t s_sum[kStepWarps + 1];
   __shared__ int s_seq;
   __shared__ int64_t s_base;
+  __shared__ StepSeq s_first;
   __shared__ float s_m[kStepWarps][kStepRows], s_l[kStepWarps][kStepRows];
   __shared__ float2 s_join[kStepRows];
   __shared__ int s_last;
   const AttnArgs& a = p.a;
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
 
-  // Tiles before each thread's run of sequences, and in all.
+  // Tiles before each thread's run of sequences, and in all.  One sequence a
+  // thread at most is the usual case: its numbers are read once.
   const int per = (a.sequences + kStepThreads - 1) / kStepThreads;
   const int q0 = tid * per;
   const int q1 = min(a.sequences, q0 + per);
   int64_t mine = 0;
-  for (int s = q0; s < q1; ++s) mine += step_seq(p, s).tiles * a.kv_heads;
+  StepSeq own{};
+  for (int s = q0; s < q1; ++s) {
+    own = step_seq(p, s);
+    mine += own.tiles * a.kv_heads;
+  }
   int64_t scan = mine;
 #pragma unroll
   for (int o = 1; o < 32; o *= 2) {
@@ -195,19 +208,20 @@ __global__ void __launch_bounds__(kStepThreads, kStepCtasPerSm) k_attn_step(cons
     total += s_sum[w];
   }
   // CTAs in use: every one of them has a tile.
-  const int64_t wanted = (total + p.min_tiles - 1) / p.min_tiles;
-  const int64_t ctas = wanted < gridDim.x ? wanted : gridDim.x;
+  const int64_t ctas = total < gridDim.x ? total : gridDim.x;
   if (blockIdx.x >= ctas) return;
-  const int64_t w0 = blockIdx.x * total / ctas, w1 = (blockIdx.x + 1) * total / ctas;
+  const int64_t w0 = share_of(blockIdx.x, total, ctas), w1 = share_of(blockIdx.x + 1, total, ctas);
   if (w0 >= before && w0 < before + mine) {
     int64_t at = before;
     int s = q0;
-    while (true) {
-      const int64_t n = step_seq(p, s).tiles * a.kv_heads;
+    while (per > 1) {
+      own = step_seq(p, s);
+      const int64_t n = own.tiles * a.kv_heads;
       if (w0 < at + n) break;
       at += n;
       ++s;
     }
+    s_first = own;
     s_seq = s;
     s_base = at;
   }
@@ -224,10 +238,12 @@ __global__ void __launch_bounds__(kStepThreads, kStepCtasPerSm) k_attn_step(cons
 
   StepCursor cur;
   cur.s = s_seq;
-  cur.q = step_seq(p, cur.s);
+  cur.q = s_first;
   {
     const int64_t at = w0 - s_base;
-    cur.head = static_cast<int>(at / cur.q.tiles);
+    cur.head = static_cast<int>(at >> 32 == 0 ? static_cast<uint32_t>(at) /
+                                                    static_cast<uint32_t>(cur.q.tiles)
+                                              : at / cur.q.tiles);
     cur.tile = at - cur.head * cur.q.tiles;
   }
   int64_t seg_first = w0 - cur.tile;  // the current segment's first tile in the whole list
@@ -616,7 +632,6 @@ cudaError_t launch_attn_step(const AttnArgs& a, const AttnWork& w, cudaStream_t 
   p.arrived = w.counters;
   p.scale_log2 = a.scale * 1.4426950408889634f;
   p.group = a.q_heads / a.kv_heads;
-  p.min_tiles = 2;
   if (a.dtype == PSPML_DTYPE_F16)
     return dp == 64 ? step_launch<__half, 64>(p, grid, s) : step_launch<__half, 128>(p, grid, s);
   return dp == 64 ? step_launch<__nv_bfloat16, 64>(p, grid, s)

@@ -11,7 +11,6 @@ PspmlError.
 from __future__ import annotations
 
 import ctypes
-import math
 import struct
 
 import numpy as np
@@ -41,11 +40,13 @@ def _on(device: int, t: torch.Tensor, what: str) -> None:
         raise ValueError(f"{what} is on {t.device}, the context on cuda:{device}")
 
 
-# struct pspml_heads as bytes: half the cost of filling a ctypes.Structure.
+# struct pspml_heads and pspml_attention_desc as bytes: half the cost of filling a
+# ctypes.Structure.
 _pack_heads = struct.Struct("@Pqqiiiifi").pack
+_pack_desc = struct.Struct("@fiii").pack
 
 
-def heads(x, device: int, what: str = "tensor") -> bytes:
+def heads(x, device: int, what: str = "tensor", tokens: int | None = None) -> bytes:
     """The C view (struct pspml_heads) of a [tokens][heads][dim] tensor or a Quantised one."""
     if type(x) is Quantised:
         x, scale, zero, dtype = x.tensor, x.scale, x.zero_point, capi.DTYPE_S8
@@ -55,7 +56,9 @@ def heads(x, device: int, what: str = "tensor") -> bytes:
             raise ValueError(f"{what}: dtype {x.dtype} is not float32, float16 or bfloat16")
     if x.get_device() != device:
         _on(device, x, what)
-    _, h, d = x.shape
+    n, h, d = x.shape
+    if tokens is not None and n != tokens:
+        raise ValueError(f"{what}: {n} tokens in a call of {tokens}")
     st, sh, sd = x.stride()
     if sd != 1 and d != 1:
         raise ValueError(f"{what}: a head's elements are not contiguous")
@@ -133,24 +136,20 @@ class KvCache:
 
 
 def _tokens(x) -> int:
-    return (x.tensor if isinstance(x, Quantised) else x).shape[0]
-
-
-def _same_tokens(n: int, *xs) -> None:
-    for x in xs:
-        if x is not None and _tokens(x) != n:
-            raise ValueError(f"views of {_tokens(x)} and {n} tokens in one call")
+    return (x.tensor if type(x) is Quantised else x).shape[0]
 
 
 def rotary_apply(rotary: Rotary, positions: torch.Tensor, q, q_out, k=None, k_out=None,
                  stream: int = 0) -> None:
     """q_out, k_out = q, k turned to their int32 positions; outputs may be the inputs."""
     n, dev = _tokens(q), rotary.ctx.device
-    _same_tokens(n, q_out, k, k_out)
-    refs = [heads(x, dev, w) if x is not None else None
-            for x, w in ((q, "q"), (q_out, "q_out"), (k, "k"), (k_out, "k_out"))]
-    capi.call("pspml_rotary_apply", rotary.handle, n,
-              _index(positions, torch.int32, n, dev, "positions"), *refs, stream)
+    status = rotary.ctx.lib.pspml_rotary_apply(
+        rotary.handle, n, _index(positions, torch.int32, n, dev, "positions"),
+        heads(q, dev, "q"), heads(q_out, dev, "q_out", n),
+        heads(k, dev, "k", n) if k is not None else None,
+        heads(k_out, dev, "k_out", n) if k_out is not None else None, stream)
+    if status:
+        capi.check(status, "pspml_rotary_apply")
 
 
 def rotary_append(rotary: Rotary, positions: torch.Tensor, slots: torch.Tensor, q, q_out, k, v,
@@ -158,23 +157,22 @@ def rotary_append(rotary: Rotary, positions: torch.Tensor, slots: torch.Tensor, 
     """q_out = q turned to its positions (q and q_out may be None); token t's turned k and its v
     go to slot slots[t] = page * page_size + slot of the cache (int64; outside it: skipped)."""
     n, dev = _tokens(k), rotary.ctx.device
-    _same_tokens(n, q, q_out, v)
     _on(dev, cache.k, "cache")
-    refs = [heads(x, dev, w) if x is not None else None
-            for x, w in ((q, "q"), (q_out, "q_out"), (k, "k"), (v, "v"))]
-    capi.call("pspml_rotary_append", rotary.handle, n,
-              _index(positions, torch.int32, n, dev, "positions"),
-              _index(slots, torch.int64, n, dev, "slots"), *refs, _ref(cache.view), stream)
+    status = rotary.ctx.lib.pspml_rotary_append(
+        rotary.handle, n, _index(positions, torch.int32, n, dev, "positions"),
+        _index(slots, torch.int64, n, dev, "slots"),
+        heads(q, dev, "q", n) if q is not None else None,
+        heads(q_out, dev, "q_out", n) if q_out is not None else None,
+        heads(k, dev, "k"), heads(v, dev, "v", n), _ref(cache.view), stream)
+    if status:
+        capi.check(status, "pspml_rotary_append")
 
 
-def _desc(dim: int, causal: bool, window: int, scale: float | None) -> capi.AttentionDesc:
-    return capi.AttentionDesc(1.0 / math.sqrt(dim) if scale is None else scale,
-                              1 if causal else 0, window, 0)
+def _desc(dim: int, causal: bool, window: int, scale: float | None) -> bytes:
+    return _pack_desc(dim ** -0.5 if scale is None else scale, 1 if causal else 0, window, 0)
 
 
-def _lse(lse, q, dev) -> int | None:
-    if lse is None:
-        return None
+def _lse(lse, q, dev) -> int:
     return _index(lse, torch.float32, q.shape[0] * q.shape[1], dev, "lse")
 
 
@@ -182,14 +180,16 @@ def prompt(ctx: capi.Context, q, k, v, starts: torch.Tensor, out, lse=None, caus
            window: int = 0, scale: float | None = None, stream: int = 0) -> None:
     """Attention over packed whole prompts: sequence s is tokens starts[s] .. starts[s+1] (int32)
     of q, k, v and out; scale defaults to dim ** -0.5; lse [tokens][heads] float32 or None."""
-    n, dev = q.shape[0], ctx.device
-    _same_tokens(n, k, v, out)
-    d = _desc(q.shape[2], causal, window, scale)
-    capi.call("pspml_attention_prompt", ctx.handle, _ref(d), n, starts.numel() - 1,
-              _index(starts, torch.int32, starts.numel(), dev, "starts"),
-              heads(q, dev, "q"), heads(k, dev, "k"),
-              heads(v, dev, "v"), heads(out, dev, "out"),
-              _lse(lse, q, dev), stream)
+    dev = ctx.device
+    n, _, dim = q.shape
+    edges = starts.numel()
+    status = ctx.lib.pspml_attention_prompt(
+        ctx.handle, _desc(dim, causal, window, scale), n, edges - 1,
+        _index(starts, torch.int32, edges, dev, "starts"), heads(q, dev, "q"),
+        heads(k, dev, "k", n), heads(v, dev, "v", n), heads(out, dev, "out", n),
+        None if lse is None else _lse(lse, q, dev), stream)
+    if status:
+        capi.check(status, "pspml_attention_prompt")
 
 
 def cached(ctx: capi.Context, q, cache: KvCache, starts: torch.Tensor, lengths: torch.Tensor,
@@ -198,17 +198,19 @@ def cached(ctx: capi.Context, q, cache: KvCache, starts: torch.Tensor, lengths: 
     """Attention of each sequence's new tokens starts[s] .. starts[s+1] of q, at most max_new,
     over its lengths[s] cached keys (the new ones among them), found through row s of the int32
     page table `pages`."""
-    n, dev = q.shape[0], ctx.device
-    _same_tokens(n, out)
+    dev = ctx.device
+    n, _, dim = q.shape
+    seqs = starts.numel() - 1
     _on(dev, cache.k, "cache")
     _on(dev, pages, "pages")
-    seqs = starts.numel() - 1
-    if pages.dtype != torch.int32 or pages.dim() != 2 or pages.shape[0] != seqs or \
-            not pages.is_contiguous():
+    if pages.dtype is not torch.int32 or pages.dim() != 2 or not pages.is_contiguous() or \
+            pages.shape[0] != seqs:
         raise ValueError("pages: needs a contiguous int32 row for each sequence")
-    d = _desc(q.shape[2], causal, window, scale)
-    capi.call("pspml_attention_cached", ctx.handle, _ref(d), n, seqs, max_new,
-              _index(starts, torch.int32, seqs + 1, dev, "starts"),
-              _index(lengths, torch.int32, seqs, dev, "lengths"), pages.data_ptr(), pages.shape[1],
-              heads(q, dev, "q"), _ref(cache.view),
-              heads(out, dev, "out"), _lse(lse, q, dev), stream)
+    status = ctx.lib.pspml_attention_cached(
+        ctx.handle, _desc(dim, causal, window, scale), n, seqs, max_new,
+        _index(starts, torch.int32, seqs + 1, dev, "starts"),
+        _index(lengths, torch.int32, seqs, dev, "lengths"), pages.data_ptr(), pages.shape[1],
+        heads(q, dev, "q"), _ref(cache.view), heads(out, dev, "out", n),
+        None if lse is None else _lse(lse, q, dev), stream)
+    if status:
+        capi.check(status, "pspml_attention_cached")
