@@ -395,7 +395,7 @@ typedef struct pspml_rotary pspml_rotary;
  * times a frequency wraps exactly, so angles lose nothing at any position.
  * Needs no device. */
 int pspml_rotary_frequencies(const pspml_rotary_desc* d, uint64_t* host_out);
-/* A rotation kept on the context's device. */
+/* A rotation kept on the context's device; it may outlive the context. */
 int pspml_rotary_create(pspml_ctx* ctx, const pspml_rotary_desc* d, pspml_rotary** out);
 int pspml_rotary_destroy(pspml_rotary* r);
 

@@ -10,8 +10,11 @@
 #include "../../include/pspml.h"
 #include "runtime.h"
 
+// Keeps what it needs of its context, so that it may be used and destroyed
+// after it.
 struct pspml_rotary {
-  pspml_ctx* ctx = nullptr;
+  int device = 0;
+  int num_sms = 0;
   pspml_rotary_desc d{};
   unsigned long long* freq = nullptr;  // device: rot_dim/2 turns per position, 64-bit fractions
 };

@@ -316,7 +316,8 @@ int pspml_rotary_create(pspml_ctx* ctx, const pspml_rotary_desc* d, pspml_rotary
   if ((st = cuda_status(cudaSetDevice(ctx->device), "cudaSetDevice"))) return st;
   auto* r = new (std::nothrow) pspml_rotary();
   if (r == nullptr) return set_error(PSPML_ERR_OOM, "host allocation failed");
-  r->ctx = ctx;
+  r->device = ctx->device;
+  r->num_sms = ctx->num_sms;
   r->d = *d;
   unsigned long long f[kMaxRotaryDim / 2];
   const size_t bytes = d->rot_dim / 2 * sizeof(f[0]);
@@ -341,7 +342,7 @@ int pspml_rotary_create(pspml_ctx* ctx, const pspml_rotary_desc* d, pspml_rotary
 
 int pspml_rotary_destroy(pspml_rotary* r) {
   if (r == nullptr) return PSPML_OK;
-  cudaSetDevice(r->ctx->device);
+  cudaSetDevice(r->device);
   if (r->freq) cudaFree(r->freq);
   delete r;
   return PSPML_OK;
@@ -368,8 +369,8 @@ int pspml_rotary_apply(pspml_rotary* r, int64_t tokens, const int32_t* positions
   a.q = view_of(q, q_out);
   a.k = view_of(k, k_out);
   fill_rotary(r, tokens, positions, q, q_out->dtype, &a);
-  if ((st = cuda_status(cudaSetDevice(r->ctx->device), "cudaSetDevice"))) return st;
-  return cuda_status(launch_rotary(a, r->ctx->num_sms, static_cast<cudaStream_t>(stream)),
+  if ((st = cuda_status(cudaSetDevice(r->device), "cudaSetDevice"))) return st;
+  return cuda_status(launch_rotary(a, r->num_sms, static_cast<cudaStream_t>(stream)),
                      "rotary launch");
 }
 
@@ -409,8 +410,8 @@ int pspml_rotary_append(pspml_rotary* r, int64_t tokens, const int32_t* position
   a.page_size = cache->page_size;
   a.slots_total = cache->pages * cache->page_size;
   fill_rotary(r, tokens, positions, k, cache->dtype, &a);
-  if ((st = cuda_status(cudaSetDevice(r->ctx->device), "cudaSetDevice"))) return st;
-  return cuda_status(launch_rotary(a, r->ctx->num_sms, static_cast<cudaStream_t>(stream)),
+  if ((st = cuda_status(cudaSetDevice(r->device), "cudaSetDevice"))) return st;
+  return cuda_status(launch_rotary(a, r->num_sms, static_cast<cudaStream_t>(stream)),
                      "rotary launch");
 }
 

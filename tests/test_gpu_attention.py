@@ -505,6 +505,19 @@ def test_python_refusals(ctx, at):
         at.rotary_apply(r, pos, q, q.as_strided((4, 2, 64), (64, 256, 1)))
 
 
+def test_rotary_outlives_its_context(ctx, at):
+    from pspml import capi
+    with capi.Context(0) as other:
+        r = at.Rotary(other, 64)
+    q = _rand(_gen(23), 3, 2, 64)
+    pos = torch.arange(3, dtype=torch.int32, device="cuda")
+    out, want = torch.empty_like(q), torch.empty_like(q)
+    at.rotary_apply(r, pos, q, out)
+    r.close()
+    at.rotary_apply(at.Rotary(ctx, 64), pos, q, want)  # no error is left behind either
+    assert torch.equal(out, want)
+
+
 def test_nothing_to_do(ctx, at):
     empty = torch.zeros((0, 2, 64), device="cuda", dtype=F16)
     at.prompt(ctx, empty, empty, empty, _starts([0]), empty.clone())
