@@ -985,9 +985,14 @@ int pow2_gcd128(int x) {
 // What the tensor maps and tiles cover beyond the vector form: a group of at
 // most 128 heads, a positive scale (the running maximum is taken over
 // unscaled products), pages of whole 8-row swizzle groups and strides that
-// are not 0 (a broadcast view).
+// are not 0 (a broadcast view) and below a tensor map's 2^40 bytes.
 bool attn_tc_covers(const AttnArgs& a) {
-  if (a.q_heads / a.kv_heads > 128 || !(a.scale > 0.0f)) return false;
+  const int64_t most = int64_t{1} << 39;  // elements of 2 bytes
+  const int64_t group = a.q_heads / a.kv_heads;
+  if (a.q_token >= most || a.q_head >= most / group || a.kv_token >= most || a.kv_head >= most ||
+      a.v_token >= most || a.v_head >= most || a.page_stride >= most)
+    return false;
+  if (group > 128 || !(a.scale > 0.0f)) return false;
   if (a.paged && (a.page_size % 8 != 0 || a.n_pages == 0)) return false;
   if ((a.tokens > 1 && a.q_token == 0) || (a.q_heads > 1 && a.q_head == 0)) return false;
   if (a.kv_heads > 1 && (a.kv_head == 0 || a.v_head == 0)) return false;
