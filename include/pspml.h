@@ -321,10 +321,12 @@ int pspml_forward_timed(pspml_model* m, const int8_t* dev_in, int8_t* dev_out,
  * counterpart in the reference.  Device pointers except where a comment says
  * "host"; asynchronous on `stream`.
  *
- * Calls of one context that use its workspace (pspml_attention_cached and
- * pspml_attention_prompt) are ordered after one another by the library when
- * they are given different streams.  Under stream capture that ordering is
- * the caller's: replays of graphs that share a context run one at a time. */
+ * The first pspml_attention_* call of a context allocates about 40 MB for
+ * the pieces of calls that are split over the device; make it before any
+ * stream capture.  Later calls allocate nothing.  Calls of one context on
+ * different streams share that memory and are ordered after one another by
+ * the library; under capture the order is the caller's: replays of graphs
+ * that share a context run one at a time. */
 typedef enum pspml_dtype {
   PSPML_DTYPE_F32 = 0,
   PSPML_DTYPE_F16 = 1,

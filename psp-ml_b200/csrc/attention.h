@@ -119,14 +119,19 @@ struct RotaryArgs {
 
 // What a split call may use between its CTAs.
 struct AttnWork {
-  uint8_t* base;        // workspace
-  size_t bytes;
+  uint8_t* base;        // attn_workspace_bytes(num_sms)
   unsigned* counters;   // kAttnCounters words, zero between calls
   unsigned* err;        // the context's device error word
   int num_sms;
 };
 
 cudaError_t launch_rotary(const RotaryArgs& a, int num_sms, cudaStream_t s);
+// Two pieces a CTA, one CTA an SM, of 256 rows of 128 sums, a maximum and a
+// sum (attn_tc.cu; the 16-row pieces of attn_step.cu need less).
+inline size_t attn_workspace_bytes(int num_sms) {
+  return static_cast<size_t>(2 * num_sms) * 256 * (128 * sizeof(float) + sizeof(float2));
+}
+
 cudaError_t launch_attn_any(const AttnArgs& a, cudaStream_t s);
 cudaError_t launch_attn_step(const AttnArgs& a, const AttnWork& w, cudaStream_t s);
 bool attn_tc_covers(const AttnArgs& a);

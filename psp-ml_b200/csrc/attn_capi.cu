@@ -251,21 +251,28 @@ bool vector_form(const AttnArgs& a) {
           a.o_token | a.o_head) % 8 == 0;
 }
 
-// Calls that use the workspace run one after another even when they are
-// given different streams.  Under capture an event of the outside cannot be
-// waited for: there the caller keeps the order.
+// Split calls of one context run one after another even when they are given
+// different streams, since they share its workspace.  Under capture an event
+// of the outside cannot be waited for: there the caller keeps the order.
 int with_workspace(pspml_ctx* ctx, const AttnArgs& a, cudaStream_t s,
                    cudaError_t (*launch)(const AttnArgs&, const AttnWork&, cudaStream_t)) {
-  AttnWork w;
-  w.base = ctx->workspace;
-  w.bytes = ctx->workspace_bytes;
-  w.counters = ctx->dev_err + 64;
-  w.err = ctx->dev_err;
-  w.num_sms = ctx->num_sms;
   cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
   int st = cuda_status(cudaStreamIsCapturing(s, &capture), "cudaStreamIsCapturing");
   if (st) return st;
   const bool order = capture == cudaStreamCaptureStatusNone;
+  if (ctx->attn_workspace == nullptr) {
+    if (!order)
+      return set_error(PSPML_ERR_UNSUPPORTED,
+                       "attention: a context's first call allocates and cannot be captured");
+    if ((st = cuda_status(cudaMalloc(&ctx->attn_workspace, attn_workspace_bytes(ctx->num_sms)),
+                          "cudaMalloc(attention workspace)")))
+      return st;
+  }
+  AttnWork w;
+  w.base = ctx->attn_workspace;
+  w.counters = ctx->dev_err + 64;
+  w.err = ctx->dev_err;
+  w.num_sms = ctx->num_sms;
   if (order && ctx->attn_used && ctx->attn_stream != s &&
       (st = cuda_status(cudaStreamWaitEvent(s, ctx->attn_done, 0), "cudaStreamWaitEvent")))
     return st;

@@ -36,6 +36,7 @@ constexpr int kStepWarps = 4;
 constexpr int kStepTile = 64;   // keys, 16 per warp
 constexpr int kStepRows = 16;
 constexpr int kStepCtasPerSm = 2;
+static_assert(kStepCtasPerSm * kStepRows <= 256, "pieces fit the attention workspace");
 
 struct StepArgs {
   AttnArgs a;
@@ -620,11 +621,7 @@ cudaError_t step_launch(const StepArgs& p, int grid, cudaStream_t s) {
 
 cudaError_t launch_attn_step(const AttnArgs& a, const AttnWork& w, cudaStream_t s) {
   const int dp = a.dim <= 64 ? 64 : 128;
-  const size_t slot = kStepRows * (dp * sizeof(float) + sizeof(float2));
-  const int64_t fit = static_cast<int64_t>(w.bytes / (2 * slot));
-  const int grid = static_cast<int>(std::min<int64_t>(
-      {static_cast<int64_t>(w.num_sms) * kStepCtasPerSm, kAttnCounters, fit}));
-  if (grid < 1) return cudaErrorMemoryAllocation;
+  const int grid = std::min(w.num_sms * kStepCtasPerSm, kAttnCounters);
   StepArgs p{};
   p.a = a;
   p.part_o = reinterpret_cast<float*>(w.base);

@@ -1025,17 +1025,13 @@ cudaError_t launch_attn_tc(const AttnArgs& a, const AttnWork& w, cudaStream_t s)
   if (p.items > 0x7FFFFFFF) return cudaErrorInvalidValue;
   // Fewer than kItemsPerSm items an SM leave some SMs idle at the end: equal
   // shares then, as long as a warp can count a sequence's key tiles quickly.
-  const int64_t slot = 256 * (dp * static_cast<int64_t>(sizeof(float)) + sizeof(float2));
   const int64_t seq_tokens = a.paged ? std::min<int64_t>(a.tokens, a.max_new) : a.tokens;
   const int64_t most_keys = a.paged ? a.pages_stride * a.page_size : a.tokens;
   int64_t grid = std::min<int64_t>(w.num_sms, kAttnCounters - 2);
   p.shares = p.items < static_cast<int64_t>(kItemsPerSm) * grid &&
-             seq_tokens / pair_tokens < kCountedPairs && 2 * slot <= static_cast<int64_t>(w.bytes) &&
-             most_keys > kMinShare * kKeys;
+             seq_tokens / pair_tokens < kCountedPairs && most_keys > kMinShare * kKeys;
   if (p.shares) {
-    grid = std::min(grid, static_cast<int64_t>(w.bytes) / (2 * slot));
     grid = std::min(grid, p.items * ((most_keys + kMinShare * kKeys - 1) / (kMinShare * kKeys)));
-    grid = std::max<int64_t>(grid, 1);
   } else {
     grid = std::min(grid, p.items);
   }

@@ -256,6 +256,7 @@ int pspml_ctx_destroy(pspml_ctx* ctx) {
   if (ctx->stream) cudaStreamDestroy(ctx->stream);
   if (ctx->attn_done) cudaEventDestroy(ctx->attn_done);
   if (ctx->workspace) cudaFree(ctx->workspace);
+  if (ctx->attn_workspace) cudaFree(ctx->attn_workspace);
   if (ctx->dev_err) cudaFree(ctx->dev_err);
   delete ctx;
   return PSPML_OK;

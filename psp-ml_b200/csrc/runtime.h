@@ -24,8 +24,9 @@ struct pspml_ctx {
   uint8_t* workspace = nullptr;     // per-op prepared tables (folded bias, requant)
   size_t workspace_bytes = 0;
   cudaStream_t stream = nullptr;    // internal stream for synchronous work
-  // Last attention call that used the workspace: a call on another stream
-  // waits for it.
+  // Pieces of split attention calls, allocated by the first such call, and
+  // the last call that used them: one on another stream waits for it.
+  uint8_t* attn_workspace = nullptr;
   cudaEvent_t attn_done = nullptr;
   cudaStream_t attn_stream = nullptr;
   bool attn_used = false;

@@ -479,6 +479,25 @@ def test_cached_in_a_graph(ctx, at, bound):
         assert torch.equal(out, first)
 
 
+def test_first_call_of_a_context_cannot_be_captured(at):
+    from pspml import capi
+    c = _Paged(_gen(24), [60], 1, 64, 16, BF16, "slots")
+    q = _rand(_gen(25), 1, 2, 64, dtype=BF16)
+    out = torch.zeros_like(q)
+    with capi.Context(0) as own:
+        args = (own, q, at.KvCache(c.k, c.v), _starts([1]), c.lengths, c.table, out, 1)
+        s = torch.cuda.Stream()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=s):
+            with pytest.raises(capi.PspmlError, match="UNSUPPORTED.*captured"):
+                at.cached(*args, stream=s.cuda_stream)
+        at.cached(*args, stream=s.cuda_stream)
+        torch.cuda.synchronize()
+        w = ref.attend(q, c.keys[0], c.values[0], 59, True, 0, 0.125)
+        _close(out, w[0], w[2], "after a refused capture")
+
+
 def test_python_refusals(ctx, at):
     q = torch.zeros((4, 2, 64), device="cuda", dtype=F16)
     starts = _starts([4])
