@@ -43,10 +43,6 @@
 
 namespace pspml {
 
-CUresult encode_tensor_map(CUtensorMap* map, const void* base, int rank, const uint64_t* dims,
-                           const uint64_t* strides_bytes, const uint32_t* box,
-                           const uint32_t* elem_strides, CUtensorMapSwizzle swizzle);
-
 namespace {
 
 // Three warpgroups: 168 registers a thread at launch, of which the softmax
@@ -156,6 +152,11 @@ __device__ __forceinline__ void store8(const AttnArgs& a, int64_t at, const floa
   }
 }
 
+// The n lowest bits, n cut to 0 .. 32.
+__device__ __forceinline__ uint32_t low_bits(int n) {
+  return n <= 0 ? 0u : (n >= 32 ? ~0u : (1u << n) - 1u);
+}
+
 // Sixteen (or, at the end of a head, eight) neighbouring outputs of a row; as
 // one 32-byte sector where the view's alignment allows it.
 template <typename T>
@@ -243,7 +244,8 @@ __device__ __forceinline__ TcGeometry tc_geometry(const TcArgs& p, const SeqSpan
   }
   g.hi_all = g.tokens1 > 0 ? hi1 : hi0;
   g.tiles0 = hi0 > g.lo ? static_cast<int>((hi0 - g.start + kKeys - 1) / kKeys) : 0;
-  g.tiles1 = g.tokens1 > 0 && hi1 > g.lo ? static_cast<int>((hi1 - g.start + kKeys - 1) / kKeys) : 0;
+  g.tiles1 =
+      g.tokens1 > 0 && hi1 > g.lo ? static_cast<int>((hi1 - g.start + kKeys - 1) / kKeys) : 0;
   return g;
 }
 
@@ -347,357 +349,358 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 
   if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
-  if (warp == 8) {
-    // ------------------------------------------------- items and TMA loads
-    const int boxes = kKeys / p.box_keys;  // one per lane
-    int slot = 0, landings = 0, issued = 0, q_loads = 0;
-    uint32_t phase = 0;
-    bool ok = true;
-    int64_t next = blockIdx.x;  // handed out: the item
-    int seq = 0, head = 0, tile = 0;
-    int64_t pair = 0;
-    SeqSpan span{0, 0, 0};
-    int64_t total = 0, at = 0, stop = 0, ctas = 0;  // shares: key tiles, this CTA's, CTAs in use
-    if (p.shares) {
-      for (int s0 = 0; s0 < a.sequences; s0 += 32) {
-        int64_t u = s0 + lane < a.sequences ? tc_seq_units(p, seq_span(a, s0 + lane)) : 0;
-#pragma unroll
-        for (int o = 16; o > 0; o /= 2) u += __shfl_xor_sync(~0u, u, o);
-        total += u * a.kv_heads;
-      }
-      const int64_t wanted = (total + kMinShare - 1) / kMinShare;
-      ctas = wanted < gridDim.x ? wanted : gridDim.x;
-      if (blockIdx.x < ctas) {
-        at = blockIdx.x * total / ctas;
-        stop = (blockIdx.x + 1) * total / ctas;
-        // The sequence, pair, head and tile that the share begins with.
-        int64_t before = 0;
-        for (int s0 = 0;; s0 += 32) {
-          SeqSpan sp{0, 0, 0};
-          if (s0 + lane < a.sequences) sp = seq_span(a, s0 + lane);
-          int64_t scan = tc_seq_units(p, sp) * a.kv_heads;
-#pragma unroll
-          for (int o = 1; o < 32; o *= 2) {
-            const int64_t v = __shfl_up_sync(~0u, scan, o);
-            if (lane >= o) scan += v;
-          }
-          const unsigned past = __ballot_sync(~0u, at < before + scan);
-          if (past != 0) {
-            const int who = __ffs(past) - 1;
-            seq = s0 + who;
-            span.begin = __shfl_sync(~0u, sp.begin, who);
-            span.keys = __shfl_sync(~0u, sp.keys, who);
-            span.rows = __shfl_sync(~0u, sp.rows, who);
-            if (who > 0) before += __shfl_sync(~0u, scan, who - 1);
-            break;
-          }
-          before += __shfl_sync(~0u, scan, 31);
-        }
-        pair = static_cast<int64_t>(tc_pairs(p, span)) - 1;
-        while (true) {
-          const int u = tc_units(tc_geometry(p, span, pair));
-          if (at < before + static_cast<int64_t>(u) * a.kv_heads) {
-            head = static_cast<int>((at - before) / u);
-            tile = static_cast<int>((at - before) - static_cast<int64_t>(head) * u);
-            break;
-          }
-          before += static_cast<int64_t>(u) * a.kv_heads;
-          --pair;
-        }
-      }
-    }
-    for (int it = 0;; ++it) {
-      TcItem* const d = &items[it & 1];
-      if (it >= 2 && !mbar_wait(&item_empty[it & 1], static_cast<uint32_t>(((it >> 1) - 1) & 1),
-                                nullptr, kItemLimitNs)) {
-        tc_fail(p.err, abort, kDevErrTmaWait);
-        ok = false;
-      }
-      bool have = __all_sync(~0u, ok && !*abort);
+    if (warp == 8) {
+      // ------------------------------------------------- items and TMA loads
+      const int boxes = kKeys / p.box_keys;  // one per lane
+      int slot = 0, landings = 0, issued = 0, q_loads = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      int64_t next = blockIdx.x;  // handed out: the item
+      int seq = 0, head = 0, tile = 0;
+      int64_t pair = 0;
+      SeqSpan span{0, 0, 0};
+      int64_t total = 0, at = 0, stop = 0, ctas = 0;  // shares: key tiles, this CTA's, CTAs in use
       if (p.shares) {
-        have = have && at < stop;
-      } else {
-        head = static_cast<int>(next % a.kv_heads);
-        have = have && next < p.items &&
-               tc_locate(p, next / a.kv_heads, lane, &seq, &pair, &span);
-      }
-      if (!have) {
-        if (lane == 0) {
-          d->end = 1;
-          mbar_arrive(&item_full[it & 1]);
+        for (int s0 = 0; s0 < a.sequences; s0 += 32) {
+          int64_t u = s0 + lane < a.sequences ? tc_seq_units(p, seq_span(a, s0 + lane)) : 0;
+#pragma unroll
+          for (int o = 16; o > 0; o /= 2) u += __shfl_xor_sync(~0u, u, o);
+          total += u * a.kv_heads;
         }
-        break;
-      }
-      const TcGeometry g = tc_geometry(p, span, pair);
-      const int64_t lo = g.lo, start = g.start, hi_all = g.hi_all;
-      const int units = tc_units(g), j0 = tile;
-      int j1 = units, pieces = 1, first_cta = 0;
-      if (p.shares) {
-        if (stop - at < j1 - j0) j1 = j0 + static_cast<int>(stop - at);
-        if (j0 > 0 || j1 < units) {
-          // Tile f of the list belongs to CTA ((f + 1) * ctas - 1) / total.
-          const int64_t f = at - j0;
-          first_cta = static_cast<int>(((f + 1) * ctas - 1) / total);
-          pieces = static_cast<int>(((f + units) * ctas - 1) / total) - first_cta + 1;
+        const int64_t wanted = (total + kMinShare - 1) / kMinShare;
+        ctas = wanted < gridDim.x ? wanted : gridDim.x;
+        if (blockIdx.x < ctas) {
+          at = blockIdx.x * total / ctas;
+          stop = (blockIdx.x + 1) * total / ctas;
+          // The sequence, pair, head and tile that the share begins with.
+          int64_t before = 0;
+          for (int s0 = 0;; s0 += 32) {
+            SeqSpan sp{0, 0, 0};
+            if (s0 + lane < a.sequences) sp = seq_span(a, s0 + lane);
+            int64_t scan = tc_seq_units(p, sp) * a.kv_heads;
+#pragma unroll
+            for (int o = 1; o < 32; o *= 2) {
+              const int64_t v = __shfl_up_sync(~0u, scan, o);
+              if (lane >= o) scan += v;
+            }
+            const unsigned past = __ballot_sync(~0u, at < before + scan);
+            if (past != 0) {
+              const int who = __ffs(past) - 1;
+              seq = s0 + who;
+              span.begin = __shfl_sync(~0u, sp.begin, who);
+              span.keys = __shfl_sync(~0u, sp.keys, who);
+              span.rows = __shfl_sync(~0u, sp.rows, who);
+              if (who > 0) before += __shfl_sync(~0u, scan, who - 1);
+              break;
+            }
+            before += __shfl_sync(~0u, scan, 31);
+          }
+          pair = static_cast<int64_t>(tc_pairs(p, span)) - 1;
+          while (true) {
+            const int u = tc_units(tc_geometry(p, span, pair));
+            if (at < before + static_cast<int64_t>(u) * a.kv_heads) {
+              head = static_cast<int>((at - before) / u);
+              tile = static_cast<int>((at - before) - static_cast<int64_t>(head) * u);
+              break;
+            }
+            before += static_cast<int64_t>(u) * a.kv_heads;
+            --pair;
+          }
         }
       }
-      const int n0 = max(0, min(j1, g.tiles0) - j0), n1 = max(0, min(j1, g.tiles1) - j0);
-      const int n = max(n0, n1);
-      if (lane == 0) {
-        d->row0 = g.row0;
-        d->place0 = g.place0;
-        d->keys = g.keys;
-        d->lo = lo;
-        d->start = start;
-        d->hi_all = hi_all;
-        d->tokens[0] = g.tokens0;
-        d->tokens[1] = g.tokens1;
-        d->n[0] = n0;
-        d->n[1] = n1;
-        d->j0 = j0;
-        d->head = head;
-        d->pieces = pieces;
-        d->first_cta = first_cta;
-        d->end = 0;
-        mbar_arrive(&item_full[it & 1]);
-      }
-      __syncwarp();
-      // The next item: asked for now, looked at when this one's loads are out.
-      unsigned taken = 0;
-      const bool more = !p.shares && p.items > gridDim.x;
-      if (more && lane == 0) taken = atomicAdd(p.next, 1u);
-
-      const int32_t* table = a.paged ? a.pages + seq * a.pages_stride : nullptr;
-      auto page_of = [&](int j) -> int {
-        const int64_t key = start + static_cast<int64_t>(j) * kKeys + lane * p.box_keys;
-        if (!a.paged || lane >= boxes || key + p.box_keys <= lo || key >= hi_all) return -1;
-        return table[static_cast<uint32_t>(key) / static_cast<uint32_t>(a.page_size)];
-      };
-      int page = n > 0 ? page_of(j0) : -1;
-      if (n > 0) {
-        if (q_loads > 0 && !mbar_wait(&q_empty, static_cast<uint32_t>((q_loads - 1) & 1), abort)) {
+      for (int it = 0;; ++it) {
+        TcItem* const d = &items[it & 1];
+        if (it >= 2 && !mbar_wait(&item_empty[it & 1], static_cast<uint32_t>(((it >> 1) - 1) & 1),
+                                  nullptr, kItemLimitNs)) {
           tc_fail(p.err, abort, kDevErrTmaWait);
           ok = false;
         }
-        __syncwarp();
+        bool have = __all_sync(~0u, ok && !*abort);
+        if (p.shares) {
+          have = have && at < stop;
+        } else {
+          head = static_cast<int>(next % a.kv_heads);
+          have = have && next < p.items &&
+                 tc_locate(p, next / a.kv_heads, lane, &seq, &pair, &span);
+        }
+        if (!have) {
+          if (lane == 0) {
+            d->end = 1;
+            mbar_arrive(&item_full[it & 1]);
+          }
+          break;
+        }
+        const TcGeometry g = tc_geometry(p, span, pair);
+        const int64_t lo = g.lo, start = g.start, hi_all = g.hi_all;
+        const int units = tc_units(g), j0 = tile;
+        int j1 = units, pieces = 1, first_cta = 0;
+        if (p.shares) {
+          if (stop - at < j1 - j0) j1 = j0 + static_cast<int>(stop - at);
+          if (j0 > 0 || j1 < units) {
+            // Tile f of the list belongs to CTA ((f + 1) * ctas - 1) / total.
+            const int64_t f = at - j0;
+            first_cta = static_cast<int>(((f + 1) * ctas - 1) / total);
+            pieces = static_cast<int>(((f + units) * ctas - 1) / total) - first_cta + 1;
+          }
+        }
+        const int n0 = max(0, min(j1, g.tiles0) - j0), n1 = max(0, min(j1, g.tiles1) - j0);
+        const int n = max(n0, n1);
         if (lane == 0) {
-          const int active = (n0 > 0) + (n1 > 0);
-          mbar_arrive_expect_tx(
-              &q_full, static_cast<uint32_t>(active * Sh::kHalves * p.tile_tokens * p.group * 128));
-          for (int t = 0; t < 2; ++t) {
-            if ((t == 0 ? n0 : n1) == 0) continue;
-            for (int h = 0; h < Sh::kHalves; ++h)
-              tma_load_4d(sq + t * Sh::kTileBytes + h * 16384, &map_q, &q_full, h * 128, 0, head,
-                          static_cast<int32_t>(g.row0 + t * p.tile_tokens));
-          }
+          d->row0 = g.row0;
+          d->place0 = g.place0;
+          d->keys = g.keys;
+          d->lo = lo;
+          d->start = start;
+          d->hi_all = hi_all;
+          d->tokens[0] = g.tokens0;
+          d->tokens[1] = g.tokens1;
+          d->n[0] = n0;
+          d->n[1] = n1;
+          d->j0 = j0;
+          d->head = head;
+          d->pieces = pieces;
+          d->first_cta = first_cta;
+          d->end = 0;
+          mbar_arrive(&item_full[it & 1]);
         }
-        ++q_loads;
-      }
-      for (int j = j0; j < j0 + n && ok; ++j) {
-        const int64_t kb = start + static_cast<int64_t>(j) * kKeys;
-        const int lo_k = v_lo(lo, start, j), hi_k = v_hi(hi_all, start, j);
-        const int first = lane * p.box_keys;
-        const bool load = lane < boxes && first < hi_k && first + p.box_keys > lo_k;
-        const int n_load = __popc(__ballot_sync(~0u, load));
-        const uint32_t bytes = static_cast<uint32_t>(n_load * p.box_keys * 128 * Sh::kHalves);
-        const int next_page = j + 1 < j0 + n ? page_of(j + 1) : -1;
-        const int32_t c2 = a.paged ? static_cast<int32_t>(static_cast<uint32_t>(kb + first) %
-                                                          static_cast<uint32_t>(a.page_size))
-                                   : static_cast<int32_t>(span.begin + kb + first);
-        const int32_t c3 = a.paged ? page : 0;
-        for (int which = 0; which < 2; ++which) {
-          const bool got = mbar_wait(&kv_empty[slot], phase ^ 1u, abort);
-          if (!got) tc_fail(p.err, abort, kDevErrTmaWait);
-          if (!__all_sync(~0u, got)) {
+        __syncwarp();
+        // The next item: asked for now, looked at when this one's loads are out.
+        unsigned taken = 0;
+        const bool more = !p.shares && p.items > gridDim.x;
+        if (more && lane == 0) taken = atomicAdd(p.next, 1u);
+
+        const int32_t* table = a.paged ? a.pages + seq * a.pages_stride : nullptr;
+        auto page_of = [&](int j) -> int {
+          const int64_t key = start + static_cast<int64_t>(j) * kKeys + lane * p.box_keys;
+          if (!a.paged || lane >= boxes || key + p.box_keys <= lo || key >= hi_all) return -1;
+          return table[static_cast<uint32_t>(key) / static_cast<uint32_t>(a.page_size)];
+        };
+        int page = n > 0 ? page_of(j0) : -1;
+        if (n > 0) {
+          const uint32_t q_phase = static_cast<uint32_t>((q_loads - 1) & 1);
+          if (q_loads > 0 && !mbar_wait(&q_empty, q_phase, abort)) {
+            tc_fail(p.err, abort, kDevErrTmaWait);
             ok = false;
-            break;
           }
-          uint8_t* dst = slots + slot * Sh::kTileBytes;
-          const bool mend = which == 1 && ((lo_k | hi_k) & 15) != 0;
-          uint64_t* bar = mend ? &landed : &kv_full[slot];
-          if (lane == 0) mbar_arrive_expect_tx(bar, bytes);
           __syncwarp();
-          if (load)
-            for (int h = 0; h < Sh::kHalves; ++h)
-              tma_load_4d(dst + h * 16384 + first * 128, which ? &map_v : &map_k, bar, h * 128,
-                          head, c2, c3);
-          __syncwarp();
-          if (mend) {
-            if (!mbar_wait(&landed, static_cast<uint32_t>(landings & 1), abort)) {
-              tc_fail(p.err, abort, kDevErrTmaWait);
+          if (lane == 0) {
+            const int boxes_q = ((n0 > 0) + (n1 > 0)) * Sh::kHalves;
+            mbar_arrive_expect_tx(
+                &q_full, static_cast<uint32_t>(boxes_q * p.tile_tokens * p.group * 128));
+            for (int t = 0; t < 2; ++t) {
+              if ((t == 0 ? n0 : n1) == 0) continue;
+              for (int h = 0; h < Sh::kHalves; ++h)
+                tma_load_4d(sq + t * Sh::kTileBytes + h * 16384, &map_q, &q_full, h * 128, 0, head,
+                            static_cast<int32_t>(g.row0 + t * p.tile_tokens));
+            }
+          }
+          ++q_loads;
+        }
+        for (int j = j0; j < j0 + n && ok; ++j) {
+          const int64_t kb = start + static_cast<int64_t>(j) * kKeys;
+          const int lo_k = v_lo(lo, start, j), hi_k = v_hi(hi_all, start, j);
+          const int first = lane * p.box_keys;
+          const bool load = lane < boxes && first < hi_k && first + p.box_keys > lo_k;
+          const int n_load = __popc(__ballot_sync(~0u, load));
+          const uint32_t bytes = static_cast<uint32_t>(n_load * p.box_keys * 128 * Sh::kHalves);
+          const int next_page = j + 1 < j0 + n ? page_of(j + 1) : -1;
+          const int32_t c2 = a.paged ? static_cast<int32_t>(static_cast<uint32_t>(kb + first) %
+                                                            static_cast<uint32_t>(a.page_size))
+                                     : static_cast<int32_t>(span.begin + kb + first);
+          const int32_t c3 = a.paged ? page : 0;
+          for (int which = 0; which < 2; ++which) {
+            const bool got = mbar_wait(&kv_empty[slot], phase ^ 1u, abort);
+            if (!got) tc_fail(p.err, abort, kDevErrTmaWait);
+            if (!__all_sync(~0u, got)) {
               ok = false;
+              break;
             }
-            ++landings;
-            const int a0 = lo_k & ~15, a1 = (hi_k + 15) & ~15;
-            const int dead = (lo_k - a0) + (a1 - hi_k);
-            for (int u = lane; u < dead * 8 * Sh::kHalves; u += 32) {
-              const int i = u / (8 * Sh::kHalves), c = u % (8 * Sh::kHalves);
-              const int r = i < lo_k - a0 ? a0 + i : hi_k + (i - (lo_k - a0));
-              *reinterpret_cast<uint4*>(dst + (c / 8) * 16384 + r * 128 + (c % 8) * 16) =
-                  make_uint4(0, 0, 0, 0);
-            }
-            fence_async_smem();
+            uint8_t* dst = slots + slot * Sh::kTileBytes;
+            const bool mend = which == 1 && ((lo_k | hi_k) & 15) != 0;
+            uint64_t* bar = mend ? &landed : &kv_full[slot];
+            if (lane == 0) mbar_arrive_expect_tx(bar, bytes);
             __syncwarp();
-            if (lane == 0) mbar_arrive(&kv_full[slot]);
+            if (load)
+              for (int h = 0; h < Sh::kHalves; ++h)
+                tma_load_4d(dst + h * 16384 + first * 128, which ? &map_v : &map_k, bar, h * 128,
+                            head, c2, c3);
+            __syncwarp();
+            if (mend) {
+              if (!mbar_wait(&landed, static_cast<uint32_t>(landings & 1), abort)) {
+                tc_fail(p.err, abort, kDevErrTmaWait);
+                ok = false;
+              }
+              ++landings;
+              const int a0 = lo_k & ~15, a1 = (hi_k + 15) & ~15;
+              const int dead = (lo_k - a0) + (a1 - hi_k);
+              for (int u = lane; u < dead * 8 * Sh::kHalves; u += 32) {
+                const int i = u / (8 * Sh::kHalves), c = u % (8 * Sh::kHalves);
+                const int r = i < lo_k - a0 ? a0 + i : hi_k + (i - (lo_k - a0));
+                *reinterpret_cast<uint4*>(dst + (c / 8) * 16384 + r * 128 + (c % 8) * 16) =
+                    make_uint4(0, 0, 0, 0);
+              }
+              fence_async_smem();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(&kv_full[slot]);
+            }
+            ++issued;
+            if (++slot == Sh::kSlots) {
+              slot = 0;
+              phase ^= 1u;
+            }
           }
-          ++issued;
-          if (++slot == Sh::kSlots) {
-            slot = 0;
-            phase ^= 1u;
-          }
+          ok = __all_sync(~0u, ok);
+          page = next_page;
         }
-        ok = __all_sync(~0u, ok);
-        page = next_page;
-      }
-      if (!p.shares) {
-        next = more ? static_cast<int64_t>(__shfl_sync(~0u, taken, 0)) + gridDim.x : p.items;
-        continue;
-      }
-      at += j1 - j0;
-      tile = j1 < units ? j1 : 0;
-      if (tile == 0 && ++head == a.kv_heads) {
-        head = 0;
-        if (--pair < 0)
-          while (++seq < a.sequences) {
-            span = seq_span(a, seq);
-            pair = static_cast<int64_t>(tc_pairs(p, span)) - 1;
-            if (pair >= 0) break;
-          }
-      }
-    }
-    if (__any_sync(~0u, *abort)) {  // the copies in flight land before the CTA leaves
-      if (q_loads > 0) mbar_wait(&q_full, static_cast<uint32_t>((q_loads - 1) & 1), nullptr);
-      if (landings > 0) mbar_wait(&landed, static_cast<uint32_t>((landings - 1) & 1), nullptr);
-      for (int i = issued > Sh::kSlots ? issued - Sh::kSlots : 0; i < issued; ++i)
-        mbar_wait(&kv_full[i % Sh::kSlots], static_cast<uint32_t>((i / Sh::kSlots) & 1), nullptr);
-    }
-    __syncwarp();
-  } else if (warp == 9) {
-    // --------------------------------------------------------------- MMAs
-    // The whole warp walks the loop and its waits; elect.sync names the one
-    // lane that issues, which is how the compiler knows that the operands of
-    // an MMA are one thread's and moves them to the tensor core directly.
-    {
-      constexpr int kFmt = std::is_same<T, __half>::value ? 0 : 1;
-      const int k_steps = (a.dim + 15) / 16;
-      const uint32_t id_qk = make_idesc_f16(128, kKeys, kFmt, 0);
-      const uint32_t id_pv = make_idesc_f16(128, k_steps * 16, kFmt, 1);
-      const uint32_t q_addr = smem_u32(sq), kv_addr = smem_u32(slots);
-      // A wait that gives up only raises the abort flag, after which every
-      // other wait ends at once.
-      auto wait = [&](uint64_t* bar, uint32_t phase) {
-        if (!mbar_wait_poll(bar, phase, abort)) tc_fail(p.err, abort, kDevErrMmaWait);
-        __syncwarp();
-      };
-      // Descriptors are built once a tile; a step adds its 16-byte units to
-      // the address, which stays within its 14 bits.  `freed`: the slot
-      // whose last reader this product is.
-      auto qk = [&](int t, int slot, uint64_t* freed) {
-        tc_fence_after();
-        if (elect_one()) {
-          const uint64_t q = make_sdesc(q_addr + t * Sh::kTileBytes, 16, 1024, 2);
-          const uint64_t b = make_sdesc(kv_addr + slot * Sh::kTileBytes, 16, 1024, 2);
-#pragma unroll
-          for (int k = 0; k < DP / 16; ++k) {
-            const int off = (k / 4) * 1024 + (k % 4) * 2;
-            if (k < k_steps)
-              umma_f16(tmem + Sh::kS + t * 128, q + off, b + off, id_qk, k > 0 ? 1u : 0u);
-          }
-          umma_commit(&s_full[t]);
-          if (freed != nullptr) umma_commit(freed);
+        if (!p.shares) {
+          next = more ? static_cast<int64_t>(__shfl_sync(~0u, taken, 0)) + gridDim.x : p.items;
+          continue;
         }
-        __syncwarp();
-      };
-      // P comes in pieces: the product of one runs while the next one's
-      // weights are found.
-      auto pv = [&](int t, int i, int slot, int k0, int k1, uint64_t* freed) {
-#pragma unroll
-        for (int h = 0; h < kPieces; ++h) {
-          prob_wait(t, h);
+        at += j1 - j0;
+        tile = j1 < units ? j1 : 0;
+        if (tile == 0 && ++head == a.kv_heads) {
+          head = 0;
+          if (--pair < 0)
+            while (++seq < a.sequences) {
+              span = seq_span(a, seq);
+              pair = static_cast<int64_t>(tc_pairs(p, span)) - 1;
+              if (pair >= 0) break;
+            }
+        }
+      }
+      if (__any_sync(~0u, *abort)) {  // the copies in flight land before the CTA leaves
+        if (q_loads > 0) mbar_wait(&q_full, static_cast<uint32_t>((q_loads - 1) & 1), nullptr);
+        if (landings > 0) mbar_wait(&landed, static_cast<uint32_t>((landings - 1) & 1), nullptr);
+        for (int i = issued > Sh::kSlots ? issued - Sh::kSlots : 0; i < issued; ++i)
+          mbar_wait(&kv_full[i % Sh::kSlots], static_cast<uint32_t>((i / Sh::kSlots) & 1), nullptr);
+      }
+      __syncwarp();
+    } else if (warp == 9) {
+      // --------------------------------------------------------------- MMAs
+      // The whole warp walks the loop and its waits; elect.sync names the one
+      // lane that issues, which is how the compiler knows that the operands of
+      // an MMA are one thread's and moves them to the tensor core directly.
+      {
+        constexpr int kFmt = std::is_same<T, __half>::value ? 0 : 1;
+        const int k_steps = (a.dim + 15) / 16;
+        const uint32_t id_qk = make_idesc_f16(128, kKeys, kFmt, 0);
+        const uint32_t id_pv = make_idesc_f16(128, k_steps * 16, kFmt, 1);
+        const uint32_t q_addr = smem_u32(sq), kv_addr = smem_u32(slots);
+        // A wait that gives up only raises the abort flag, after which every
+        // other wait ends at once.
+        auto wait = [&](uint64_t* bar, uint32_t phase) {
+          if (!mbar_wait_poll(bar, phase, abort)) tc_fail(p.err, abort, kDevErrMmaWait);
+          __syncwarp();
+        };
+        // Descriptors are built once a tile; a step adds its 16-byte units to
+        // the address, which stays within its 14 bits.  `freed`: the slot
+        // whose last reader this product is.
+        auto qk = [&](int t, int slot, uint64_t* freed) {
           tc_fence_after();
           if (elect_one()) {
-            const uint64_t b = make_sdesc(kv_addr + slot * Sh::kTileBytes, 16384, 1024, 2);
-            const uint32_t o = tmem + Sh::kO + t * DP, a = tmem + Sh::kS + t * 128;
+            const uint64_t q = make_sdesc(q_addr + t * Sh::kTileBytes, 16, 1024, 2);
+            const uint64_t b = make_sdesc(kv_addr + slot * Sh::kTileBytes, 16, 1024, 2);
 #pragma unroll
-            for (int k = h * (8 / kPieces); k < (h + 1) * (8 / kPieces); ++k)
-              if (k >= k0 && k < k1)
-                umma_f16_ta(o, a + k * 8, b + k * 128, id_pv, i > 0 || k > k0 ? 1u : 0u);
-            if (h == kPieces - 1) {
-              umma_commit(&o_done[t]);
-              if (freed != nullptr) umma_commit(freed);
+            for (int k = 0; k < DP / 16; ++k) {
+              const int off = (k / 4) * 1024 + (k % 4) * 2;
+              if (k < k_steps)
+                umma_f16(tmem + Sh::kS + t * 128, q + off, b + off, id_qk, k > 0 ? 1u : 0u);
             }
+            umma_commit(&s_full[t]);
+            if (freed != nullptr) umma_commit(freed);
           }
           __syncwarp();
-        }
-      };
-      uint32_t done[2] = {0, 0};   // key tiles of A and of B so far
-      int k_slot = 0, q_items = 0; // ring slot and phase of the next key tile
-      uint32_t k_phase = 0;
-      for (int it = 0;; ++it) {
-        const TcItem* const d = take(it);
-        if (d == nullptr || d->end) break;
-        const int n0 = d->n[0], n1 = d->n[1], n = max(n0, n1);
-        if (n > 0) {
-          const int k_first = v_lo(d->lo, d->start, d->j0) / 16;  // steps of the first key tile
-          const int k_last = (v_hi(d->hi_all, d->start, d->j0 + n - 1) + 15) / 16;  // of the last
-          wait(&q_full, static_cast<uint32_t>(q_items & 1));
-          ++q_items;
-          wait(&kv_full[k_slot], k_phase);
+        };
+        // P comes in pieces: the product of one runs while the next one's
+        // weights are found.
+        auto pv = [&](int t, int i, int slot, int k0, int k1, uint64_t* freed) {
 #pragma unroll
-          for (int t = 0; t < 2; ++t) {
-            const int nt = t == 0 ? n0 : n1;
-            if (nt == 0) continue;
-            if (done[t] > 0) wait(&o_done[t], (done[t] - 1) & 1u);
-            qk(t, k_slot, t == 0 && n1 > 0 ? nullptr : &kv_empty[k_slot]);
-          }
-          if (n == 1) {
-            if (elect_one()) umma_commit(&q_empty);
+          for (int h = 0; h < kPieces; ++h) {
+            prob_wait(t, h);
+            tc_fence_after();
+            if (elect_one()) {
+              const uint64_t b = make_sdesc(kv_addr + slot * Sh::kTileBytes, 16384, 1024, 2);
+              const uint32_t o = tmem + Sh::kO + t * DP, a = tmem + Sh::kS + t * 128;
+#pragma unroll
+              for (int k = h * (8 / kPieces); k < (h + 1) * (8 / kPieces); ++k)
+                if (k >= k0 && k < k1)
+                  umma_f16_ta(o, a + k * 8, b + k * 128, id_pv, i > 0 || k > k0 ? 1u : 0u);
+              if (h == kPieces - 1) {
+                umma_commit(&o_done[t]);
+                if (freed != nullptr) umma_commit(freed);
+              }
+            }
             __syncwarp();
           }
-          for (int i = 0; i < n; ++i) {
-            int v_slot = k_slot + 1;
-            uint32_t v_phase = k_phase;
-            if (v_slot == Sh::kSlots) {
-              v_slot = 0;
-              v_phase ^= 1u;
-            }
-            k_slot = v_slot + 1;
-            k_phase = v_phase;
-            if (k_slot == Sh::kSlots) {
-              k_slot = 0;
-              k_phase ^= 1u;
-            }
-            wait(&kv_full[v_slot], v_phase);
-            if (i + 1 < n) wait(&kv_full[k_slot], k_phase);
-            const int k0 = i == 0 ? k_first : 0, k1 = i == n - 1 ? k_last : kKeys / 16;
+        };
+        uint32_t done[2] = {0, 0};   // key tiles of A and of B so far
+        int k_slot = 0, q_items = 0; // ring slot and phase of the next key tile
+        uint32_t k_phase = 0;
+        for (int it = 0;; ++it) {
+          const TcItem* const d = take(it);
+          if (d == nullptr || d->end) break;
+          const int n0 = d->n[0], n1 = d->n[1], n = max(n0, n1);
+          if (n > 0) {
+            const int k_first = v_lo(d->lo, d->start, d->j0) / 16;  // steps of the first key tile
+            const int k_last = (v_hi(d->hi_all, d->start, d->j0 + n - 1) + 15) / 16;  // of the last
+            wait(&q_full, static_cast<uint32_t>(q_items & 1));
+            ++q_items;
+            wait(&kv_full[k_slot], k_phase);
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
-              const int nt = t == 0 ? n0 : n1, other = t == 0 ? n1 : 0;
-              if (i >= nt) continue;
-              pv(t, i, v_slot, k0, k1, i < other ? nullptr : &kv_empty[v_slot]);
-              if (i + 1 >= nt) continue;
-              // P is read before the next S is written over it.
-              wait(&o_done[t], (done[t] + static_cast<uint32_t>(i)) & 1u);
-              qk(t, k_slot, i + 1 < other ? nullptr : &kv_empty[k_slot]);
+              const int nt = t == 0 ? n0 : n1;
+              if (nt == 0) continue;
+              if (done[t] > 0) wait(&o_done[t], (done[t] - 1) & 1u);
+              qk(t, k_slot, t == 0 && n1 > 0 ? nullptr : &kv_empty[k_slot]);
             }
-            if (i + 2 == n) {  // the item's last scores are on their way: Q may be replaced
+            if (n == 1) {
               if (elect_one()) umma_commit(&q_empty);
               __syncwarp();
             }
+            for (int i = 0; i < n; ++i) {
+              int v_slot = k_slot + 1;
+              uint32_t v_phase = k_phase;
+              if (v_slot == Sh::kSlots) {
+                v_slot = 0;
+                v_phase ^= 1u;
+              }
+              k_slot = v_slot + 1;
+              k_phase = v_phase;
+              if (k_slot == Sh::kSlots) {
+                k_slot = 0;
+                k_phase ^= 1u;
+              }
+              wait(&kv_full[v_slot], v_phase);
+              if (i + 1 < n) wait(&kv_full[k_slot], k_phase);
+              const int k0 = i == 0 ? k_first : 0, k1 = i == n - 1 ? k_last : kKeys / 16;
+#pragma unroll
+              for (int t = 0; t < 2; ++t) {
+                const int nt = t == 0 ? n0 : n1, other = t == 0 ? n1 : 0;
+                if (i >= nt) continue;
+                pv(t, i, v_slot, k0, k1, i < other ? nullptr : &kv_empty[v_slot]);
+                if (i + 1 >= nt) continue;
+                // P is read before the next S is written over it.
+                wait(&o_done[t], (done[t] + static_cast<uint32_t>(i)) & 1u);
+                qk(t, k_slot, i + 1 < other ? nullptr : &kv_empty[k_slot]);
+              }
+              if (i + 2 == n) {  // the item's last scores are on their way: Q may be replaced
+                if (elect_one()) umma_commit(&q_empty);
+                __syncwarp();
+              }
+            }
+            done[0] += static_cast<uint32_t>(n0);
+            done[1] += static_cast<uint32_t>(n1);
           }
-          done[0] += static_cast<uint32_t>(n0);
-          done[1] += static_cast<uint32_t>(n1);
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&item_empty[it & 1]);
         }
+        // Every MMA completes before tensor memory is freed.
+        if (elect_one()) umma_commit(&drain);
         __syncwarp();
-        if (lane == 0) mbar_arrive(&item_empty[it & 1]);
+        mbar_wait(&drain, 0, nullptr);
       }
-      // Every MMA completes before tensor memory is freed.
-      if (elect_one()) umma_commit(&drain);
       __syncwarp();
-      mbar_wait(&drain, 0, nullptr);
     }
-    __syncwarp();
-  }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
     // ------------------------------------------------------------ softmax
@@ -707,227 +710,231 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     const uint32_t ts = tmem + Sh::kS + t * 128 + lanes, to = tmem + Sh::kO + t * DP + lanes;
     uint32_t done = 0;  // key tiles so far
     for (int it = 0;; ++it) {
-    const TcItem* const d = take(it);
-    if (d == nullptr || d->end) break;
-    const int nt = d->n[t];
-    // The row's keys [row_beg, row_end), and those that every row of the tile
-    // sees, counted from the part's first key tile.
-    int row_beg, row_end, all_beg, all_end;
-    {
-      const int64_t first = d->start + static_cast<int64_t>(d->j0) * kKeys;
-      const int64_t place = d->place0 + t * p.tile_tokens;  // of the tile's first token
-      auto end_of = [&](int64_t at) {
-        const int64_t e = a.causal && at + 1 < d->keys ? at + 1 : d->keys;
-        return static_cast<int>(e > first ? e - first : 0);
-      };
-      auto beg_of = [&](int64_t at) {
-        const int64_t b = a.window > 0 ? at - a.window + 1 : 0;
-        return static_cast<int>(b > first ? b - first : 0);
-      };
-      const int tok = row / p.group;
-      row_end = end_of(place + tok);
-      row_beg = beg_of(place + tok);
-      all_end = end_of(place);
-      all_beg = beg_of(place + d->tokens[t] - 1);
-    }
-    float m = -INFINITY, l = 0.0f;
-    bool ok = true;
-    for (int i = 0; i < nt; ++i) {
-      const int kb = i * kKeys;
-      if (!mbar_wait(&s_full[t], (done + static_cast<uint32_t>(i)) & 1u, abort)) {
-        tc_fail(p.err, abort, kDevErrEpiWait);
-        ok = false;
-      }
-      __syncwarp();
-      tc_fence_after();
-      uint32_t s[kKeys];
-      tmem_ld128(ts, s);
-      const bool edge = kb + kKeys > all_end || kb < all_beg;
-      if (edge) {
-        const int end = row_end - kb, beg = row_beg - kb;
-#pragma unroll
-        for (int x = 0; x < kKeys; ++x)
-          if (x >= end || x < beg) s[x] = 0xFF800000u;  // -inf
-      }
-      float top[4];
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        const uint32_t* q = s + 32 * c;
-        top[c] = fmaxf(__uint_as_float(q[0]), __uint_as_float(q[1]));
-#pragma unroll
-        for (int x = 2; x < 32; x += 2)
-          top[c] = fmaxf(fmaxf(top[c], __uint_as_float(q[x])), __uint_as_float(q[x + 1]));
-      }
-      const float m2 = fmaxf(m, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])));
-      const bool grow = (m2 - m) * p.scale_log2 > kGrowLog2;
-      if (__any_sync(~0u, grow)) {
-        const float f = grow ? tc_ex2((m - m2) * p.scale_log2) : 1.0f;
-        if (grow) m = m2;
-        l *= f;
-        if (i > 0) {
-#pragma unroll 1
-          for (int c = 0; c < DP / 32; ++c) {
-            uint32_t o[32];
-            tmem_ld32(to + c * 32, o);
-#pragma unroll
-            for (int x = 0; x < 32; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * f);
-            tmem_st32(to + c * 32, o);
-          }
-        }
-      }
-      const float base = m == -INFINITY ? 0.0f : m * p.scale_log2;
-      const uint64_t scale2 = f2(p.scale_log2, p.scale_log2), base2 = f2(-base, -base);
-      uint64_t sums[2] = {0, 0};
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        uint32_t w[16];
-#pragma unroll
-        for (int x = 0; x < 16; ++x) {
-          const uint32_t* q = s + 32 * c + 2 * x;
-          float e0, e1;
-          f2_get(f2_fma(f2(__uint_as_float(q[0]), __uint_as_float(q[1])), scale2, base2), e0, e1);
-          e0 = tc_ex2(e0);
-          e1 = tc_ex2(e1);
-          sums[x & 1] = f2_add(sums[x & 1], f2(e0, e1));
-          w[x] = pack2<T>(e0, e1);
-        }
-        tmem_st16(ts + c * 16, w);
-        if ((c + 1) % (4 / kPieces) == 0) {
-          tmem_wait_st();
-          tc_fence_before();
-          prob_arrive(t, c / (4 / kPieces));
-        }
-      }
-      float sa, sb, sc, sd;
-      f2_get(sums[0], sa, sb);
-      f2_get(sums[1], sc, sd);
-      l += (sa + sb) + (sc + sd);
-    }
-    done += static_cast<uint32_t>(nt);
-    if (nt > 0 && ok) {
-      ok = mbar_wait(&o_done[t], (done - 1) & 1u, abort);
-      if (!ok) tc_fail(p.err, abort, kDevErrEpiWait);
-      __syncwarp();
-      tc_fence_after();
-    }
-    ok = __all_sync(~0u, ok);
-    // Read back here so that the loop above does not carry them in registers.
-    const volatile TcItem* const v_item = &items[it & 1];
-    const int64_t row0 = v_item->row0;
-    const int head = v_item->head, pieces = v_item->pieces, first_cta = v_item->first_cta;
-    // This CTA's piece: it ends the CTA's share if the item begins here.
-    const int64_t slot = 2 * static_cast<int64_t>(blockIdx.x) + (v_item->j0 == 0 ? 1 : 0);
-    const int tk = row / p.group;
-    const bool real = tk < v_item->tokens[t];
-    const int64_t out_row = row0 + t * p.tile_tokens + tk;
-    const int h = head * p.group + (row - tk * p.group);
-    if (ok) {
-      const float f = pieces > 1 ? 1.0f : (l == 0.0f ? 0.0f : 1.0f / l);
-      const int64_t at = out_row * a.o_token + h * a.o_head;
-#pragma unroll 1
-      for (int c = 0; c < DP / 32; ++c) {
-        uint32_t o[32];
-        if (nt > 0) {
-          tmem_ld32(to + c * 32, o);
-        } else {
-#pragma unroll
-          for (int x = 0; x < 32; ++x) o[x] = 0;
-        }
-        float v[32];
-#pragma unroll
-        for (int x = 0; x < 32; ++x) v[x] = __uint_as_float(o[x]) * f;
-        if (real) {
-          if (pieces == 1) {
-#pragma unroll
-            for (int x = 0; x < 32; x += 16)
-              if (c * 32 + x < a.dim)
-                store16<T>(a, at + c * 32 + x, v + x, c * 32 + x + 16 <= a.dim, p.wide_out);
-          } else {
-            float4* dst = p.part_o + (slot * (DP / 4) + c * 8) * 256 + t * 128 + row;
-#pragma unroll
-            for (int x = 0; x < 8; ++x)
-              dst[x * 256] = make_float4(v[4 * x], v[4 * x + 1], v[4 * x + 2], v[4 * x + 3]);
-          }
-        }
-      }
-      const float ml = m == -INFINITY ? -INFINITY : m * p.scale_log2;
-      if (real && pieces > 1) p.part_ml[slot * 256 + t * 128 + row] = make_float2(ml, l);
-      if (real && pieces == 1 && a.lse != nullptr)
-        a.lse[out_row * a.q_heads + h] =
-            l == 0.0f ? -INFINITY : (log2f(l) + ml) * 0.69314718055994531f;
-    }
-    if (pieces > 1) {
-      __threadfence();
-      asm volatile("bar.sync 1, 256;" ::: "memory");
-      if (tid == 0) {
-        const unsigned arrived = atomicAdd(p.arrived + first_cta, 1u);
-        s_last = arrived + 1 == static_cast<unsigned>(pieces);
-        if (s_last) p.arrived[first_cta] = 0;
-      }
-      asm volatile("bar.sync 1, 256;" ::: "memory");
-      if (s_last) {
-        __threadfence();
-        // Each thread joins a row: its maximum and sum over the pieces, then
-        // its columns, kCols at a time.  A piece without a key that counts
-        // (sum 0) has nothing to add.
-        auto slot_of = [&](int x) {
-          return 2 * static_cast<int64_t>(first_cta + x) + (x == 0 ? 1 : 0);
+      const TcItem* const d = take(it);
+      if (d == nullptr || d->end) break;
+      const int nt = d->n[t];
+      // The row's keys [row_beg, row_end), and those that every row of the tile
+      // sees, counted from the part's first key tile.
+      int row_beg, row_end, all_beg, all_end;
+      {
+        const int64_t first = d->start + static_cast<int64_t>(d->j0) * kKeys;
+        const int64_t place = d->place0 + t * p.tile_tokens;  // of the tile's first token
+        auto end_of = [&](int64_t at) {
+          const int64_t e = a.causal && at + 1 < d->keys ? at + 1 : d->keys;
+          return static_cast<int>(e > first ? e - first : 0);
         };
-        const int tt = tid / 128, rr = tid % 128;
-        const int jt = rr / p.group;
-        if (jt < v_item->tokens[tt]) {
-          float mm = -INFINITY, sum = 0.0f;
-#pragma unroll 4
-          for (int x = 0; x < pieces; ++x) {
-            const float2 ml = __ldcg(p.part_ml + slot_of(x) * 256 + tid);
-            const float top = fmaxf(mm, ml.x);
-            const float bs = top == -INFINITY ? 0.0f : top;
-            sum = sum * tc_ex2(mm - bs) + ml.y * tc_ex2(ml.x - bs);
-            mm = top;
-          }
-          const float bs = mm == -INFINITY ? 0.0f : mm;
-          const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-          const int64_t orow = row0 + tt * p.tile_tokens + jt;
-          const int oh = head * p.group + (rr - jt * p.group);
-          const int64_t at = orow * a.o_token + oh * a.o_head;
-          constexpr int kCols = 32;
-#pragma unroll 1
-          for (int col = 0; col < DP; col += kCols) {
-            float acc[kCols];
+        auto beg_of = [&](int64_t at) {
+          const int64_t b = a.window > 0 ? at - a.window + 1 : 0;
+          return static_cast<int>(b > first ? b - first : 0);
+        };
+        const int tok = row / p.group;
+        row_end = end_of(place + tok);
+        row_beg = beg_of(place + tok);
+        all_end = end_of(place);
+        all_beg = beg_of(place + d->tokens[t] - 1);
+      }
+      float m = -INFINITY, l = 0.0f;
+      bool ok = true;
+      for (int i = 0; i < nt; ++i) {
+        const int kb = i * kKeys;
+        if (!mbar_wait(&s_full[t], (done + static_cast<uint32_t>(i)) & 1u, abort)) {
+          tc_fail(p.err, abort, kDevErrEpiWait);
+          ok = false;
+        }
+        __syncwarp();
+        tc_fence_after();
+        uint32_t s[kKeys];
+        tmem_ld128(ts, s);
+        const bool edge = kb + kKeys > all_end || kb < all_beg;
+        if (edge) {
+          const int end = row_end - kb, beg = row_beg - kb;
 #pragma unroll
-            for (int y = 0; y < kCols; ++y) acc[y] = 0.0f;
-#pragma unroll 2
+          for (int c = 0; c < 4; ++c) {
+            const uint32_t seen = low_bits(end - 32 * c) & ~low_bits(beg - 32 * c);
+#pragma unroll
+            for (int x = 0; x < 32; ++x)
+              if ((seen >> x & 1u) == 0) s[32 * c + x] = 0xFF800000u;  // -inf
+          }
+        }
+        float top[4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const uint32_t* q = s + 32 * c;
+          top[c] = fmaxf(__uint_as_float(q[0]), __uint_as_float(q[1]));
+#pragma unroll
+          for (int x = 2; x < 32; x += 2)
+            top[c] = fmaxf(fmaxf(top[c], __uint_as_float(q[x])), __uint_as_float(q[x + 1]));
+        }
+        const float m2 = fmaxf(m, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])));
+        const bool grow = (m2 - m) * p.scale_log2 > kGrowLog2;
+        if (__any_sync(~0u, grow)) {
+          const float f = grow ? tc_ex2((m - m2) * p.scale_log2) : 1.0f;
+          if (grow) m = m2;
+          l *= f;
+          if (i > 0) {
+#pragma unroll 1
+            for (int c = 0; c < DP / 32; ++c) {
+              uint32_t o[32];
+              tmem_ld32(to + c * 32, o);
+#pragma unroll
+              for (int x = 0; x < 32; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * f);
+              tmem_st32(to + c * 32, o);
+            }
+          }
+        }
+        const float base = m == -INFINITY ? 0.0f : m * p.scale_log2;
+        const uint64_t scale2 = f2(p.scale_log2, p.scale_log2), base2 = f2(-base, -base);
+        uint64_t sums[2] = {0, 0};
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          uint32_t w[16];
+#pragma unroll
+          for (int x = 0; x < 16; ++x) {
+            const uint32_t* q = s + 32 * c + 2 * x;
+            float e0, e1;
+            f2_get(f2_fma(f2(__uint_as_float(q[0]), __uint_as_float(q[1])), scale2, base2), e0, e1);
+            e0 = tc_ex2(e0);
+            e1 = tc_ex2(e1);
+            sums[x & 1] = f2_add(sums[x & 1], f2(e0, e1));
+            w[x] = pack2<T>(e0, e1);
+          }
+          tmem_st16(ts + c * 16, w);
+          if ((c + 1) % (4 / kPieces) == 0) {
+            tmem_wait_st();
+            tc_fence_before();
+            prob_arrive(t, c / (4 / kPieces));
+          }
+        }
+        float sa, sb, sc, sd;
+        f2_get(sums[0], sa, sb);
+        f2_get(sums[1], sc, sd);
+        l += (sa + sb) + (sc + sd);
+      }
+      done += static_cast<uint32_t>(nt);
+      if (nt > 0 && ok) {
+        ok = mbar_wait(&o_done[t], (done - 1) & 1u, abort);
+        if (!ok) tc_fail(p.err, abort, kDevErrEpiWait);
+        __syncwarp();
+        tc_fence_after();
+      }
+      ok = __all_sync(~0u, ok);
+      // Read back here so that the loop above does not carry them in registers.
+      const volatile TcItem* const v_item = &items[it & 1];
+      const int64_t row0 = v_item->row0;
+      const int head = v_item->head, pieces = v_item->pieces, first_cta = v_item->first_cta;
+      // This CTA's piece: it ends the CTA's share if the item begins here.
+      const int64_t slot = 2 * static_cast<int64_t>(blockIdx.x) + (v_item->j0 == 0 ? 1 : 0);
+      const int tk = row / p.group;
+      const bool real = tk < v_item->tokens[t];
+      const int64_t out_row = row0 + t * p.tile_tokens + tk;
+      const int h = head * p.group + (row - tk * p.group);
+      if (ok) {
+        const float f = pieces > 1 ? 1.0f : (l == 0.0f ? 0.0f : 1.0f / l);
+        const int64_t at = out_row * a.o_token + h * a.o_head;
+#pragma unroll 1
+        for (int c = 0; c < DP / 32; ++c) {
+          uint32_t o[32];
+          if (nt > 0) {
+            tmem_ld32(to + c * 32, o);
+          } else {
+#pragma unroll
+            for (int x = 0; x < 32; ++x) o[x] = 0;
+          }
+          float v[32];
+#pragma unroll
+          for (int x = 0; x < 32; ++x) v[x] = __uint_as_float(o[x]) * f;
+          if (real) {
+            if (pieces == 1) {
+#pragma unroll
+              for (int x = 0; x < 32; x += 16)
+                if (c * 32 + x < a.dim)
+                  store16<T>(a, at + c * 32 + x, v + x, c * 32 + x + 16 <= a.dim, p.wide_out);
+            } else {
+              float4* dst = p.part_o + (slot * (DP / 4) + c * 8) * 256 + t * 128 + row;
+#pragma unroll
+              for (int x = 0; x < 8; ++x)
+                dst[x * 256] = make_float4(v[4 * x], v[4 * x + 1], v[4 * x + 2], v[4 * x + 3]);
+            }
+          }
+        }
+        const float ml = m == -INFINITY ? -INFINITY : m * p.scale_log2;
+        if (real && pieces > 1) p.part_ml[slot * 256 + t * 128 + row] = make_float2(ml, l);
+        if (real && pieces == 1 && a.lse != nullptr)
+          a.lse[out_row * a.q_heads + h] =
+              l == 0.0f ? -INFINITY : (log2f(l) + ml) * 0.69314718055994531f;
+      }
+      if (pieces > 1) {
+        __threadfence();
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+        if (tid == 0) {
+          const unsigned arrived = atomicAdd(p.arrived + first_cta, 1u);
+          s_last = arrived + 1 == static_cast<unsigned>(pieces);
+          if (s_last) p.arrived[first_cta] = 0;
+        }
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+        if (s_last) {
+          __threadfence();
+          // Each thread joins a row: its maximum and sum over the pieces, then
+          // its columns, kCols at a time.  A piece without a key that counts
+          // (sum 0) has nothing to add.
+          auto slot_of = [&](int x) {
+            return 2 * static_cast<int64_t>(first_cta + x) + (x == 0 ? 1 : 0);
+          };
+          const int tt = tid / 128, rr = tid % 128;
+          const int jt = rr / p.group;
+          if (jt < v_item->tokens[tt]) {
+            float mm = -INFINITY, sum = 0.0f;
+#pragma unroll 4
             for (int x = 0; x < pieces; ++x) {
               const float2 ml = __ldcg(p.part_ml + slot_of(x) * 256 + tid);
-              const float f = tc_ex2(ml.x - bs);
-              float4 v[kCols / 4];
-#pragma unroll
-              for (int y = 0; y < kCols / 4; ++y)
-                v[y] = __ldcg(p.part_o + (slot_of(x) * (DP / 4) + col / 4 + y) * 256 + tid);
-              if (ml.y != 0.0f)
-#pragma unroll
-                for (int y = 0; y < kCols / 4; ++y) {
-                  acc[4 * y] = fmaf(v[y].x, f, acc[4 * y]);
-                  acc[4 * y + 1] = fmaf(v[y].y, f, acc[4 * y + 1]);
-                  acc[4 * y + 2] = fmaf(v[y].z, f, acc[4 * y + 2]);
-                  acc[4 * y + 3] = fmaf(v[y].w, f, acc[4 * y + 3]);
-                }
+              const float top = fmaxf(mm, ml.x);
+              const float bs = top == -INFINITY ? 0.0f : top;
+              sum = sum * tc_ex2(mm - bs) + ml.y * tc_ex2(ml.x - bs);
+              mm = top;
             }
+            const float bs = mm == -INFINITY ? 0.0f : mm;
+            const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+            const int64_t orow = row0 + tt * p.tile_tokens + jt;
+            const int oh = head * p.group + (rr - jt * p.group);
+            const int64_t at = orow * a.o_token + oh * a.o_head;
+            constexpr int kCols = 32;
+#pragma unroll 1
+            for (int col = 0; col < DP; col += kCols) {
+              float acc[kCols];
 #pragma unroll
-            for (int y = 0; y < kCols; ++y) acc[y] *= inv;
+              for (int y = 0; y < kCols; ++y) acc[y] = 0.0f;
+#pragma unroll 2
+              for (int x = 0; x < pieces; ++x) {
+                const float2 ml = __ldcg(p.part_ml + slot_of(x) * 256 + tid);
+                const float f = tc_ex2(ml.x - bs);
+                float4 v[kCols / 4];
 #pragma unroll
-            for (int y = 0; y < kCols; y += 16)
-              if (col + y < a.dim)
-                store16<T>(a, at + col + y, acc + y, col + y + 16 <= a.dim, p.wide_out);
+                for (int y = 0; y < kCols / 4; ++y)
+                  v[y] = __ldcg(p.part_o + (slot_of(x) * (DP / 4) + col / 4 + y) * 256 + tid);
+                if (ml.y != 0.0f)
+#pragma unroll
+                  for (int y = 0; y < kCols / 4; ++y) {
+                    acc[4 * y] = fmaf(v[y].x, f, acc[4 * y]);
+                    acc[4 * y + 1] = fmaf(v[y].y, f, acc[4 * y + 1]);
+                    acc[4 * y + 2] = fmaf(v[y].z, f, acc[4 * y + 2]);
+                    acc[4 * y + 3] = fmaf(v[y].w, f, acc[4 * y + 3]);
+                  }
+              }
+#pragma unroll
+              for (int y = 0; y < kCols; ++y) acc[y] *= inv;
+#pragma unroll
+              for (int y = 0; y < kCols; y += 16)
+                if (col + y < a.dim)
+                  store16<T>(a, at + col + y, acc + y, col + y + 16 <= a.dim, p.wide_out);
+            }
+            if (a.lse != nullptr)
+              a.lse[orow * a.q_heads + oh] =
+                  sum == 0.0f ? -INFINITY : (log2f(sum) + bs) * 0.69314718055994531f;
           }
-          if (a.lse != nullptr)
-            a.lse[orow * a.q_heads + oh] =
-                sum == 0.0f ? -INFINITY : (log2f(sum) + bs) * 0.69314718055994531f;
         }
       }
-    }
-    __syncwarp();
-    if (lane == 0) mbar_arrive(&item_empty[it & 1]);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&item_empty[it & 1]);
     }
     tc_fence_before();
   }
