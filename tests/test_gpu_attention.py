@@ -381,6 +381,74 @@ def test_cached(ctx, at, seqs, hq, hkv, dim, page, dtype, window, order):
     _check_out(again, lse, wants)
 
 
+def _check_some(out, lse, seqs, every, attend):
+    """Checks every `every`-th sequence (and the first and last ones) of many."""
+    at = 0
+    for s, n in enumerate(seqs):
+        if n and (s % every == 0 or s < 3 or s >= len(seqs) - 3):
+            _check_out(out[at:at + n], lse[at:at + n], [attend(s, at, n)])
+        at += n
+    assert at == out.shape[0] and torch.isfinite(out).all()
+
+
+@pytest.mark.parametrize("count,longest,hq,hkv,dim", [(700, 40, 4, 2, 64), (150, 300, 16, 8, 128),
+                                                      (33, 900, 6, 6, 80)])
+def test_prompt_many_sequences(ctx, at, count, longest, hq, hkv, dim):
+    # More items than CTAs: handed out by a counter that the call leaves as it found it.
+    g = _gen(30)
+    lengths = torch.randint(0, longest + 1, (count,), generator=torch.Generator().manual_seed(count))
+    lengths = lengths.tolist()
+    t = sum(lengths)
+    q, k, v = (_rand(g, t, h, dim, dtype=BF16) for h in (hq, hkv, hkv))
+    starts = _starts(lengths)
+    out, lse = torch.full_like(q, NAN), torch.full((t, hq), NAN, device="cuda")
+    for _ in range(3):
+        again = torch.full_like(q, NAN)
+        at.prompt(ctx, q, k, v, starts, again, lse=lse)
+        if torch.isfinite(out).all():
+            assert torch.equal(out, again)
+        out = again
+    ctx.check_device()
+    _check_some(out, lse, lengths, max(1, count // 8), lambda s, a, n: ref.attend(
+        q[a:a + n], k[a:a + n], v[a:a + n], 0, True, 0, dim ** -0.5))
+
+
+@pytest.mark.parametrize("count,longest,chunk,hq,hkv,dim,page,window", [
+    (700, 90, 1, 8, 2, 64, 16, 0), (300, 500, 1, 7, 1, 128, 16, 60), (40, 1500, 6, 32, 4, 128, 32, 0),
+    (9, 3000, 90, 8, 8, 64, 128, 0), (3, 4000, 200, 28, 4, 128, 16, 900), (200, 200, 30, 4, 2, 96, 8, 0)])
+def test_cached_many_sequences(ctx, at, count, longest, chunk, hq, hkv, dim, page, window):
+    g, rng = _gen(31), torch.Generator().manual_seed(count)
+    new = torch.randint(0, chunk + 1, (count,), generator=rng).tolist()
+    lengths = [n + int(torch.randint(0, longest, (1,), generator=rng)) for n in new]
+    c = _Paged(g, lengths, hkv, dim, page, F16, "slots")
+    t = sum(new)
+    q = _rand(g, t, hq, dim, dtype=F16)
+    out, lse = torch.full_like(q, NAN), torch.full((t, hq), NAN, device="cuda")
+    cache, starts = at.KvCache(c.k, c.v), _starts(new)
+    at.cached(ctx, q, cache, starts, c.lengths, c.table, out, max_new=chunk, lse=lse, window=window)
+    again = torch.full_like(q, NAN)
+    at.cached(ctx, q, cache, starts, c.lengths, c.table, again, max_new=chunk, window=window)
+    ctx.check_device()
+    assert torch.equal(out, again)
+    _check_some(out, lse, new, max(1, count // 8), lambda s, a, n: ref.attend(
+        q[a:a + n], c.keys[s], c.values[s], lengths[s] - n, True, window, dim ** -0.5))
+
+
+def test_prompt_long_split_over_the_device(ctx, at):
+    # Few items of many key tiles: cut into equal shares, pieces joined; S8 and lse as well.
+    g = _gen(32)
+    q, k, v = (_rand(g, 3000, h, 64, dtype=BF16) for h in (2, 1, 1))
+    out, lse = torch.empty_like(q), torch.empty((3000, 2), device="cuda")
+    at.prompt(ctx, q, k, v, _starts([3000]), out, lse=lse)
+    out8 = torch.empty((3000, 2, 64), dtype=torch.int8, device="cuda")
+    at.prompt(ctx, q, k, v, _starts([3000]), at.Quantised(out8, 0.004, 2))
+    rows = [0, 1, 127, 128, 500, 1023, 1024, 2047, 2500, 2998, 2999]
+    for r in rows:
+        w = ref.attend(q[r:r + 1], k, v, r, True, 0, 0.125)
+        _check_out(out[r:r + 1], lse[r:r + 1], [w])
+        _check_out(out8[r:r + 1], lse[r:r + 1], [w], 0.004, 2)
+
+
 def test_cached_not_causal(ctx, at):
     c = _Paged(_gen(12), [150, 7], 2, 64, 16, BF16, "slots")
     q = _rand(_gen(13), 12, 4, 64, dtype=BF16)
