@@ -303,7 +303,7 @@ cudaError_t launch_vec(const RotaryArgs& a, int num_sms, cudaStream_t s) {
   // the heads are spread over blocks until the machine is full of threads.
   pl.lanes = std::max(1, std::min({4, heads, kThreads / most}));
   int split = 1;
-  while (split * pl.lanes < heads &&
+  while (split * pl.lanes < heads && split < 32768 &&
          a.tokens * units * pl.lanes * split < static_cast<int64_t>(num_sms) * 1024)
     split *= 2;
   int64_t blocks = 0;
