@@ -36,6 +36,14 @@ constexpr int kStepWarps = 4;
 constexpr int kStepTile = 64;   // keys, 16 per warp
 constexpr int kStepRows = 16;
 constexpr int kStepCtasPerSm = 2;
+constexpr int kJoinDepth = 16;    // pieces whose loads are in flight in a join
+// One token over 63776 keys of one key head takes 39 us at 2, 27 at 8, 28 at
+// 32 and 33 with a piece on every CTA; over 25291 keys of two key heads 22, 16,
+// 14 and 20 (with the launch, cold caches).
+constexpr float kPieceTiles = 32;
+// Segments of so few tiles are not cut: a cut costs about 3 us, a tile 0.3 (one
+// token of 68 sequences of up to 353 keys: 16 us cut, 14 whole).
+constexpr int kWholeTiles = 8;
 static_assert(kStepCtasPerSm * kStepRows <= 256, "pieces fit the attention workspace");
 
 struct StepArgs {
@@ -173,7 +181,9 @@ template <typename T, int DP>
 __global__ void __launch_bounds__(kStepThreads, kStepCtasPerSm) k_attn_step(const StepArgs p) {
   using Sh = StepShape<DP>;
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ int64_t s_sum[kStepWarps + 1];
+  __shared__ int64_t s_sum[kStepWarps];
+  __shared__ int s_live[kStepWarps], s_longest[kStepWarps];
+  __shared__ int64_t s_begin, s_end;
   __shared__ int s_seq;
   __shared__ int64_t s_base;
   __shared__ StepSeq s_first;
@@ -189,29 +199,73 @@ __global__ void __launch_bounds__(kStepThreads, kStepCtasPerSm) k_attn_step(cons
   const int q0 = tid * per;
   const int q1 = min(a.sequences, q0 + per);
   int64_t mine = 0;
+  int rows_seqs = 0;  // sequences with rows
+  int64_t most = 0;   // tiles of the longest one
   StepSeq own{};
   for (int s = q0; s < q1; ++s) {
     own = step_seq(p, s);
     mine += own.tiles * a.kv_heads;
+    rows_seqs += own.tiles > 0;
+    most = own.tiles > most ? own.tiles : most;
   }
+  rows_seqs = __reduce_add_sync(~0u, rows_seqs);
+  const int longest = __reduce_max_sync(~0u, static_cast<int>(most));
   int64_t scan = mine;
 #pragma unroll
   for (int o = 1; o < 32; o *= 2) {
     const int64_t v = __shfl_up_sync(~0u, scan, o);
     if (lane >= o) scan += v;
   }
-  if (lane == 31) s_sum[warp] = scan;
+  if (lane == 31) {
+    s_sum[warp] = scan;
+    s_live[warp] = rows_seqs;
+    s_longest[warp] = longest;
+  }
   __syncthreads();
-  int64_t total = 0, before = scan - mine;
+  int64_t total = 0, before = scan - mine, segments = 0;
+  bool uncut = true;
 #pragma unroll
   for (int w = 0; w < kStepWarps; ++w) {
     if (w < warp) before += s_sum[w];
     total += s_sum[w];
+    segments += s_live[w];
+    uncut &= s_longest[w] <= kWholeTiles;
   }
-  // CTAs in use: every one of them has a tile.
-  const int64_t ctas = total < gridDim.x ? total : gridDim.x;
+  segments *= a.kv_heads;
+  // CTAs in use: every one of them has a tile.  A segment of T tiles in c
+  // pieces takes T / c tiles' time and then a join that grows with c, so c
+  // grows with the root of T; kPieceTiles is measured.
+  int64_t ctas = total < gridDim.x ? total : gridDim.x;
+  if (!uncut) {
+    const float best = ceilf(sqrtf(kPieceTiles * static_cast<float>(total) *
+                                   static_cast<float>(segments)));
+    if (best < static_cast<float>(ctas)) ctas = static_cast<int64_t>(best);
+  }
   if (blockIdx.x >= ctas) return;
-  const int64_t w0 = share_of(blockIdx.x, total, ctas), w1 = share_of(blockIdx.x + 1, total, ctas);
+  int64_t w0 = share_of(blockIdx.x, total, ctas), w1 = share_of(blockIdx.x + 1, total, ctas);
+  if (uncut) {
+    // Short segments stay whole: the shares' ends move to the nearest one's.
+    if (tid == 0) s_end = total;  // the last share's
+    __syncthreads();
+    for (int e = 0; e < 2; ++e) {
+      const int64_t w = e ? w1 : w0;
+      if (w < before || w >= before + mine) continue;
+      int64_t at = before;
+      int s = q0;
+      StepSeq q = own;
+      while (per > 1) {
+        q = step_seq(p, s++);
+        if (w < at + q.tiles * a.kv_heads) break;
+        at += q.tiles * a.kv_heads;
+      }
+      const int64_t in = (w - at) % q.tiles;
+      (e ? s_end : s_begin) = 2 * in < q.tiles ? w - in : w - in + q.tiles;
+    }
+    __syncthreads();
+    w0 = s_begin;
+    w1 = s_end;
+    if (w0 >= w1) return;
+  }
   if (w0 >= before && w0 < before + mine) {
     int64_t at = before;
     int s = q0;
@@ -566,7 +620,7 @@ __global__ void __launch_bounds__(kStepThreads, kStepCtasPerSm) k_attn_step(cons
             const int rr = u / (DP / 4), e = (u % (DP / 4)) * 4;
             const float2 j = s_join[rr];
             float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 8
+#pragma unroll kJoinDepth
             for (int i = 0; i < pieces; ++i) {
               const int64_t at = slot_of(i) * kStepRows + rr;
               const float f = ex2(__ldcg(&p.part_ml[at].x) - j.x);

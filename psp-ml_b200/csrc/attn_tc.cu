@@ -52,12 +52,14 @@ constexpr int kSoftmaxRegs = 200;
 constexpr int kOtherRegs = 104;
 constexpr int kKeys = 128;        // keys a tile
 constexpr int kPieces = 2;        // in which P is handed to the MMA warp
-// Calls of fewer items an SM are cut into equal shares.  Cutting costs a piece
-// written and read per cut: six tiles of work an item on 20 heads of 4001
-// tokens take 72 us whole and 104 us cut (2.8 items an SM), 80 items of up to
-// 94 key tiles 189 us whole and 131 us cut.
+// Calls of fewer items an SM count their key tiles, and are cut into equal
+// shares if the longest item has kCutTiles more than a share.  Cutting costs a
+// piece written and read per cut, about the time of as many tiles: 400 items
+// of 7 tiles on average take 72 us whole and 104 us cut, 80 items of up to 94
+// tiles 189 us whole and 131 us cut.
 constexpr int kItemsPerSm = 2;
-constexpr int kCountedPairs = 64;
+constexpr int kCutTiles = 6;
+constexpr int kCountedSequences = 4096;
 constexpr float kGrowLog2 = 8.0f; // largest stale maximum, as a power of two
 
 struct TcArgs {
@@ -254,12 +256,36 @@ __device__ __forceinline__ TcGeometry tc_geometry(const TcArgs& p, const SeqSpan
 __device__ __forceinline__ int tc_units(const TcGeometry& g) {
   return max(1, max(g.tiles0, g.tiles1));
 }
-// Key tiles of a sequence for one key head.
-__device__ __forceinline__ int64_t tc_seq_units(const TcArgs& p, const SeqSpan& sp) {
-  int64_t units = 0;
-  const int pairs = static_cast<int>(tc_pairs(p, sp));
-  for (int i = 0; i < pairs; ++i) units += tc_units(tc_geometry(p, sp, i));
-  return units;
+// The sum of `v` over the threads before this one in the block; `all`: over
+// the block.
+__device__ __forceinline__ int tc_scan(int v, int tid, int* warp_sums, int* all) {
+  const int lane = tid % 32;
+  int scan = v;
+#pragma unroll
+  for (int o = 1; o < 32; o *= 2) {
+    const int x = __shfl_up_sync(~0u, scan, o);
+    if (lane >= o) scan += x;
+  }
+  __syncthreads();  // the last scan's sums have been read
+  if (lane == 31) warp_sums[tid / 32] = scan;
+  __syncthreads();
+  int before = 0;
+  *all = 0;
+#pragma unroll
+  for (int w = 0; w < kTcThreads / 32; ++w) {
+    if (w < tid / 32) before += warp_sums[w];
+    *all += warp_sums[w];
+  }
+  return before + scan - v;
+}
+// The last of the n ascending numbers that is at most x, which the first is.
+__device__ __forceinline__ int tc_find(const int* a, int n, int64_t x, int per) {
+  int lo = 0, hi = n;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) / 2;
+    if (static_cast<int64_t>(a[mid]) * per <= x) lo = mid; else hi = mid;
+  }
+  return lo;
 }
 
 // What a CTA's warps need to know of one item, or of its part of one.
@@ -274,6 +300,14 @@ struct TcItem {
   int32_t end;         // no more items
 };
 constexpr int kMinShare = 4;     // key tiles of a share, at least
+// Where a CTA's share of the key tiles begins and ends.
+struct TcShare {
+  int64_t total = 0, at = 0, stop = 0;  // key tiles of all items; this CTA's
+  int ctas = 0;                         // CTAs in use; 0: items are handed out whole
+  int seq = 0, head = 0, tile = 0;
+  int64_t pair = 0;
+  SeqSpan span{0, 0, 0};
+};
 constexpr uint64_t kItemLimitNs = 5 * kWaitLimitNs;  // longer than any wait within an item
 
 template <typename T, int DP>
@@ -288,7 +322,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   __shared__ TcItem items[2];
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_word;
-  __shared__ int s_last;
+  __shared__ int s_last, s_longest, s_scan[kTcThreads / 32];
   const AttnArgs& a = p.a;
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
   volatile int* abort = &abort_word;
@@ -298,6 +332,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 
   if (tid == 0) {
     abort_word = 0;
+    s_longest = 0;
     mbar_init(&q_full, 1);
     mbar_init(&q_empty, 1);
     mbar_init(&landed, 1);
@@ -322,6 +357,63 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     }
     tmem_alloc(&tmem_slot, Sh::kCols);
     tmem_relinquish();
+  }
+  // Few items: their key tiles are counted, with room for the tiles as
+  // scratch.  Cutting pays where one item outlasts an equal share by more
+  // than the pieces cost.
+  TcShare share;
+  bool more = p.items > gridDim.x;  // than one item a CTA, handed out by the counter
+  if (p.shares) {
+    int* const first_pair = reinterpret_cast<int*>(sq);  // of each sequence
+    int pairs = 0, all;
+    for (int s0 = 0; s0 < a.sequences; s0 += kTcThreads) {
+      const int s = s0 + tid;
+      const int mine =
+          s < a.sequences ? static_cast<int>(tc_pairs(p, seq_span(a, s))) : 0;
+      const int before = tc_scan(mine, tid, s_scan, &all);
+      if (s < a.sequences) first_pair[s] = pairs + before;
+      pairs += all;
+    }
+    if (tid == 0) first_pair[a.sequences] = pairs;
+    __syncthreads();
+    int* const first_tile = first_pair + a.sequences + 1;  // of each pair, for one key head
+    int tiles = 0, longest = 0;
+    for (int i0 = 0; i0 < pairs; i0 += kTcThreads) {
+      const int i = i0 + tid;
+      int units = 0;
+      if (i < pairs) {
+        const int s = tc_find(first_pair, a.sequences, i, 1);
+        units = tc_units(tc_geometry(p, seq_span(a, s), first_pair[s + 1] - 1 - i));
+      }
+      const int before = tc_scan(units, tid, s_scan, &all);
+      if (i < pairs) first_tile[i] = tiles + before;
+      tiles += all;
+      longest = max(longest, units);
+    }
+    if (tid == 0) first_tile[pairs] = tiles;
+    longest = __reduce_max_sync(~0u, longest);
+    if (lane == 0) atomicMax(&s_longest, longest);
+    __syncthreads();
+    const int64_t total = static_cast<int64_t>(tiles) * a.kv_heads;
+    if (s_longest > total / gridDim.x + kCutTiles) {
+      more = false;
+      share.total = total;
+      const int64_t wanted = (total + kMinShare - 1) / kMinShare;
+      share.ctas = static_cast<int>(wanted < gridDim.x ? wanted : gridDim.x);
+      if (blockIdx.x < share.ctas) {
+        share.at = blockIdx.x * total / share.ctas;
+        share.stop = (blockIdx.x + 1) * total / share.ctas;
+        const int i = tc_find(first_tile, pairs, share.at, a.kv_heads);
+        const int units = first_tile[i + 1] - first_tile[i];
+        const int64_t in = share.at - static_cast<int64_t>(first_tile[i]) * a.kv_heads;
+        share.head = static_cast<int>(in / units);
+        share.tile = static_cast<int>(in - static_cast<int64_t>(share.head) * units);
+        share.seq = tc_find(first_pair, a.sequences, i, 1);
+        share.pair = first_pair[share.seq + 1] - 1 - i;
+        share.span = seq_span(a, share.seq);
+      }
+    }
+    fence_async_smem();  // the scratch is read before TMA writes over it
   }
   tc_fence_before();
   __syncthreads();
@@ -356,58 +448,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       uint32_t phase = 0;
       bool ok = true;
       int64_t next = blockIdx.x;  // handed out: the item
-      int seq = 0, head = 0, tile = 0;
-      int64_t pair = 0;
-      SeqSpan span{0, 0, 0};
-      int64_t total = 0, at = 0, stop = 0, ctas = 0;  // shares: key tiles, this CTA's, CTAs in use
-      if (p.shares) {
-        for (int s0 = 0; s0 < a.sequences; s0 += 32) {
-          int64_t u = s0 + lane < a.sequences ? tc_seq_units(p, seq_span(a, s0 + lane)) : 0;
-#pragma unroll
-          for (int o = 16; o > 0; o /= 2) u += __shfl_xor_sync(~0u, u, o);
-          total += u * a.kv_heads;
-        }
-        const int64_t wanted = (total + kMinShare - 1) / kMinShare;
-        ctas = wanted < gridDim.x ? wanted : gridDim.x;
-        if (blockIdx.x < ctas) {
-          at = blockIdx.x * total / ctas;
-          stop = (blockIdx.x + 1) * total / ctas;
-          // The sequence, pair, head and tile that the share begins with.
-          int64_t before = 0;
-          for (int s0 = 0;; s0 += 32) {
-            SeqSpan sp{0, 0, 0};
-            if (s0 + lane < a.sequences) sp = seq_span(a, s0 + lane);
-            int64_t scan = tc_seq_units(p, sp) * a.kv_heads;
-#pragma unroll
-            for (int o = 1; o < 32; o *= 2) {
-              const int64_t v = __shfl_up_sync(~0u, scan, o);
-              if (lane >= o) scan += v;
-            }
-            const unsigned past = __ballot_sync(~0u, at < before + scan);
-            if (past != 0) {
-              const int who = __ffs(past) - 1;
-              seq = s0 + who;
-              span.begin = __shfl_sync(~0u, sp.begin, who);
-              span.keys = __shfl_sync(~0u, sp.keys, who);
-              span.rows = __shfl_sync(~0u, sp.rows, who);
-              if (who > 0) before += __shfl_sync(~0u, scan, who - 1);
-              break;
-            }
-            before += __shfl_sync(~0u, scan, 31);
-          }
-          pair = static_cast<int64_t>(tc_pairs(p, span)) - 1;
-          while (true) {
-            const int u = tc_units(tc_geometry(p, span, pair));
-            if (at < before + static_cast<int64_t>(u) * a.kv_heads) {
-              head = static_cast<int>((at - before) / u);
-              tile = static_cast<int>((at - before) - static_cast<int64_t>(head) * u);
-              break;
-            }
-            before += static_cast<int64_t>(u) * a.kv_heads;
-            --pair;
-          }
-        }
-      }
+      const bool cut = share.ctas > 0;
+      int seq = share.seq, head = share.head, tile = share.tile;
+      int64_t pair = share.pair, at = share.at;
+      SeqSpan span = share.span;
       for (int it = 0;; ++it) {
         TcItem* const d = &items[it & 1];
         if (it >= 2 && !mbar_wait(&item_empty[it & 1], static_cast<uint32_t>(((it >> 1) - 1) & 1),
@@ -416,8 +460,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           ok = false;
         }
         bool have = __all_sync(~0u, ok && !*abort);
-        if (p.shares) {
-          have = have && at < stop;
+        if (cut) {
+          have = have && at < share.stop;
         } else {
           head = static_cast<int>(next % a.kv_heads);
           have = have && next < p.items &&
@@ -434,13 +478,13 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         const int64_t lo = g.lo, start = g.start, hi_all = g.hi_all;
         const int units = tc_units(g), j0 = tile;
         int j1 = units, pieces = 1, first_cta = 0;
-        if (p.shares) {
-          if (stop - at < j1 - j0) j1 = j0 + static_cast<int>(stop - at);
+        if (cut) {
+          if (share.stop - at < j1 - j0) j1 = j0 + static_cast<int>(share.stop - at);
           if (j0 > 0 || j1 < units) {
             // Tile f of the list belongs to CTA ((f + 1) * ctas - 1) / total.
             const int64_t f = at - j0;
-            first_cta = static_cast<int>(((f + 1) * ctas - 1) / total);
-            pieces = static_cast<int>(((f + units) * ctas - 1) / total) - first_cta + 1;
+            first_cta = static_cast<int>(((f + 1) * share.ctas - 1) / share.total);
+            pieces = static_cast<int>(((f + units) * share.ctas - 1) / share.total) - first_cta + 1;
           }
         }
         const int n0 = max(0, min(j1, g.tiles0) - j0), n1 = max(0, min(j1, g.tiles1) - j0);
@@ -466,7 +510,6 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         __syncwarp();
         // The next item: asked for now, looked at when this one's loads are out.
         unsigned taken = 0;
-        const bool more = !p.shares && p.items > gridDim.x;
         if (more && lane == 0) taken = atomicAdd(p.next, 1u);
 
         const int32_t* table = a.paged ? a.pages + seq * a.pages_stride : nullptr;
@@ -552,7 +595,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           ok = __all_sync(~0u, ok);
           page = next_page;
         }
-        if (!p.shares) {
+        if (!cut) {
           next = more ? static_cast<int64_t>(__shfl_sync(~0u, taken, 0)) + gridDim.x : p.items;
           continue;
         }
@@ -903,7 +946,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
               float acc[kCols];
 #pragma unroll
               for (int y = 0; y < kCols; ++y) acc[y] = 0.0f;
-#pragma unroll 2
+#pragma unroll 4
               for (int x = 0; x < pieces; ++x) {
                 const float2 ml = __ldcg(p.part_ml + slot_of(x) * 256 + tid);
                 const float f = tc_ex2(ml.x - bs);
@@ -945,7 +988,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   }
   // Every CTA has asked for its last item: the last one out leaves the
   // counters as it found them.
-  if (tid == 0 && !p.shares && p.items > gridDim.x && atomicAdd(p.done, 1u) + 1 == gridDim.x) {
+  if (tid == 0 && more && atomicAdd(p.done, 1u) + 1 == gridDim.x) {
     *p.next = 0;
     *p.done = 0;
   }
@@ -1030,13 +1073,12 @@ cudaError_t launch_attn_tc(const AttnArgs& a, const AttnWork& w, cudaStream_t s)
     pairs = std::min(pairs, a.sequences * ((a.max_new + pair_tokens - 1) / pair_tokens));
   p.items = pairs * a.kv_heads;
   if (p.items > 0x7FFFFFFF) return cudaErrorInvalidValue;
-  // Fewer than kItemsPerSm items an SM leave some SMs idle at the end: equal
-  // shares then, as long as a warp can count a sequence's key tiles quickly.
-  const int64_t seq_tokens = a.paged ? std::min<int64_t>(a.tokens, a.max_new) : a.tokens;
+  // Fewer than kItemsPerSm items an SM may leave some SMs idle at the end.
   const int64_t most_keys = a.paged ? a.pages_stride * a.page_size : a.tokens;
   int64_t grid = std::min<int64_t>(w.num_sms, kAttnCounters - 2);
   p.shares = p.items < static_cast<int64_t>(kItemsPerSm) * grid &&
-             seq_tokens / pair_tokens < kCountedPairs && most_keys > kMinShare * kKeys;
+             a.sequences <= kCountedSequences && most_keys > kCutTiles * kKeys &&
+             most_keys < (1 << 28);  // the count stays within 32 bits
   if (p.shares) {
     grid = std::min(grid, p.items * ((most_keys + kMinShare * kKeys - 1) / (kMinShare * kKeys)));
   } else {
