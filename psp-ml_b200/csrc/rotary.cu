@@ -9,6 +9,10 @@
 // product would be off by 6e-3 rad at position 100000.  Only the reduced
 // angle is rounded to a float; sums and products are 32-bit and rounded once
 // to the output type.
+//
+// Bytes bound it.  On a B200, cold: 16384 tokens of 40 F16 heads of 128, 64
+// turned, 56.5 us (335 MB, 5.9 TB/s); 8191 int8 tokens of 28 + 4 + 4 heads
+// appended as F16, 23.3 us (113 MB, 4.9 TB/s); 8 BF16 tokens of 40 heads 4.8 us.
 #include <cuda_runtime.h>
 
 #include <algorithm>
