@@ -420,9 +420,8 @@ int pspml_rotary_append(pspml_rotary* r, int64_t tokens, const int32_t* position
 /* Row at position p of its sequence sees the keys j of that sequence with
  * j <= p (causal) and j > p - window (window > 0, needs causal), weighted
  * by softmax(scale * q.k).  A row that sees no key gives zeros and a
- * log-sum-exp of -inf.  Keys past a sequence's end never count, whatever
- * their slots hold; a non-finite value of a sequence's own key may reach any
- * of that sequence's rows. */
+ * log-sum-exp of -inf.  What a row does not see never counts, whatever it
+ * holds: keys past a sequence's end, masked keys, other sequences. */
 typedef struct pspml_attention_desc {
   float scale;
   int32_t causal;        /* 0 / 1                                           */

@@ -16,7 +16,8 @@
 // registers, and joins its warps where a (sequence, key head) ends.  Where a
 // share cuts one, the pieces go to the workspace as unnormalised sums with
 // their maximum and sum, and the CTA that arrives last joins them in order:
-// the same bits on every call.
+// the same bits on every call.  With several new tokens, rows that come out
+// non-finite are looked at again (attn_rows.cuh).
 //
 // On a B200, cold, 32 query and 8 key heads of 128, BF16: one token over
 // 131077 keys 89 us (537 MB, 6.0 TB/s); one token of each of 64 sequences of
@@ -29,6 +30,7 @@
 #include <type_traits>
 
 #include "attention.h"
+#include "attn_rows.cuh"
 #include "ptx.cuh"
 
 namespace pspml {
@@ -181,8 +183,9 @@ __device__ __forceinline__ void store2(const AttnArgs& a, int64_t at, float x, f
   }
 }
 
-template <typename T, int DP>
-__global__ void __launch_bounds__(kStepThreads, kStepCtasPerSm) k_attn_step(const StepArgs p) {
+// kMulti: more than one new token a sequence, whose rows see different keys.
+template <typename T, int DP, bool kMulti>
+__global__ void __launch_bounds__(kStepThreads, kStepCtasPerSm) k_attn_step(const __grid_constant__ StepArgs p) {
   using Sh = StepShape<DP>;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ int64_t s_sum[kStepWarps];
@@ -194,6 +197,8 @@ __global__ void __launch_bounds__(kStepThreads, kStepCtasPerSm) k_attn_step(cons
   __shared__ float s_m[kStepWarps][kStepRows], s_l[kStepWarps][kStepRows];
   __shared__ float2 s_join[kStepRows];
   __shared__ int s_last;
+  __shared__ int s_bad;     // an output was not finite
+  __shared__ int s_joined;  // bits: the cut segment at the share's begin, at its end
   const AttnArgs& a = p.a;
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
 
@@ -220,6 +225,7 @@ __global__ void __launch_bounds__(kStepThreads, kStepCtasPerSm) k_attn_step(cons
     const int64_t v = __shfl_up_sync(~0u, scan, o);
     if (lane >= o) scan += v;
   }
+  if (tid == 0) s_bad = s_joined = 0;
   if (lane == 31) {
     s_sum[warp] = scan;
     s_live[warp] = rows_seqs;
@@ -561,12 +567,15 @@ __global__ void __launch_bounds__(kStepThreads, kStepCtasPerSm) k_attn_step(cons
             const int64_t row = cur.q.begin + tok;
             const int h = cur.head * p.group + (r - tok * p.group);
             const int64_t at = row * a.o_token + h * a.o_head;
+            float check = 0.0f;  // NaN once an output is not finite
 #pragma unroll
             for (int i = 0; i < Sh::kNB; ++i) {
               const int e = i * 8 + 2 * (lane % 4);
-              if (e < a.dim)
-                store2<T>(a, at + e, o[i][2 * x] * inv[x], o[i][2 * x + 1] * inv[x]);
+              const float lo = o[i][2 * x] * inv[x], hi = o[i][2 * x + 1] * inv[x];
+              if (e < a.dim) store2<T>(a, at + e, lo, hi);
+              if (kMulti) check = fmaf(lo, 0.0f, fmaf(hi, 0.0f, check));
             }
+            if (check != 0.0f) s_bad = 1;
             if (a.lse != nullptr && lane % 4 == 0)
               a.lse[row * a.q_heads + h] =
                   sum[x] == 0.0f ? -INFINITY : (log2f(sum[x]) + top[x]) * 0.69314718055994531f;
@@ -592,7 +601,10 @@ __global__ void __launch_bounds__(kStepThreads, kStepCtasPerSm) k_attn_step(cons
           if (lane == 0) {
             const unsigned n = atomicAdd(p.arrived + c0, 1u);
             s_last = n + 1 == static_cast<unsigned>(pieces);
-            if (s_last) p.arrived[c0] = 0;
+            if (s_last) {
+              p.arrived[c0] = 0;
+              s_joined |= seg_first < w0 ? 1 : 2;
+            }
           }
         }
         __syncthreads();
@@ -639,10 +651,17 @@ __global__ void __launch_bounds__(kStepThreads, kStepCtasPerSm) k_attn_step(cons
             const int64_t row = cur.q.begin + tok;
             const int h = cur.head * p.group + (rr - tok * p.group);
             const int64_t at = row * a.o_token + h * a.o_head + e;
+            acc.x *= inv;
+            acc.y *= inv;
+            acc.z *= inv;
+            acc.w *= inv;
             if (e < a.dim) {
-              store2<T>(a, at, acc.x * inv, acc.y * inv);
-              store2<T>(a, at + 2, acc.z * inv, acc.w * inv);
+              store2<T>(a, at, acc.x, acc.y);
+              store2<T>(a, at + 2, acc.z, acc.w);
             }
+            if (kMulti &&
+                fmaf(acc.x, 0.0f, fmaf(acc.y, 0.0f, fmaf(acc.z, 0.0f, acc.w * 0.0f))) != 0.0f)
+              s_bad = 1;
             if (a.lse != nullptr && e == 0)
               a.lse[row * a.q_heads + h] =
                   j.y == 0.0f ? -INFINITY : (log2f(j.y) + j.x) * 0.69314718055994531f;
@@ -656,9 +675,41 @@ __global__ void __launch_bounds__(kStepThreads, kStepCtasPerSm) k_attn_step(cons
     step_advance(p, cur);
   }
   cp_wait<0>();
+  if constexpr (kMulti) {
+    if (s_bad == 0) return;
+    // Once more over the segments whose outputs this CTA wrote: here, so that
+    // the loop above keeps its registers (391 us against 235 for 64 sequences
+    // of up to 8192 keys with the call inside, and 225 without it: a single
+    // token's rows see the same keys and do without).
+    cur.s = s_seq;
+    cur.q = s_first;
+    cur.head = static_cast<int>((w0 - s_base) / cur.q.tiles);
+    for (int64_t at = s_base + cur.head * cur.q.tiles; at < w1;) {
+      const int64_t end = at + cur.q.tiles;
+      if ((at >= w0 && end <= w1) || (s_joined & (at < w0 ? 1 : 2)) != 0) {
+        AttnRows r;
+        r.table = a.pages + cur.s * a.pages_stride;
+        r.begin = 0;
+        r.keys = r.hi = cur.q.keys;
+        r.lo = cur.q.lo;
+        r.row0 = cur.q.begin;
+        r.place0 = cur.q.place0;
+        r.head = cur.head;
+        r.group = p.group;
+        r.first = 0;
+        const int rows = static_cast<int>(cur.q.rows) * p.group;
+        attn_rows_again<T, DP>(a, r, ((1u << rows) - 1u) & (0xFu << (4 * warp)));
+      }
+      at = end;
+      if (++cur.head == a.kv_heads) {
+        cur.head = 0;
+        step_next_seq(p, cur);
+      }
+    }
+  }
 }
 
-template <typename T, int DP>
+template <typename T, int DP, bool kMulti>
 cudaError_t step_launch(const StepArgs& p, int grid, cudaStream_t s) {
   using Sh = StepShape<DP>;
   static std::atomic<uint64_t> attr_done{0};
@@ -667,11 +718,11 @@ cudaError_t step_launch(const StepArgs& p, int grid, cudaStream_t s) {
   const uint64_t bit = 1ull << (dev & 63);
   if ((attr_done.load() & bit) == 0) {
     const cudaError_t e = cudaFuncSetAttribute(
-        k_attn_step<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::kSmem);
+        k_attn_step<T, DP, kMulti>, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::kSmem);
     if (e != cudaSuccess) return e;
     attr_done.fetch_or(bit);
   }
-  k_attn_step<T, DP><<<grid, kStepThreads, Sh::kSmem, s>>>(p);
+  k_attn_step<T, DP, kMulti><<<grid, kStepThreads, Sh::kSmem, s>>>(p);
   return cudaGetLastError();
 }
 
@@ -687,10 +738,18 @@ cudaError_t launch_attn_step(const AttnArgs& a, const AttnWork& w, cudaStream_t 
   p.arrived = w.counters;
   p.scale_log2 = a.scale * 1.4426950408889634f;
   p.group = a.q_heads / a.kv_heads;
-  if (a.dtype == PSPML_DTYPE_F16)
-    return dp == 64 ? step_launch<__half, 64>(p, grid, s) : step_launch<__half, 128>(p, grid, s);
-  return dp == 64 ? step_launch<__nv_bfloat16, 64>(p, grid, s)
-                  : step_launch<__nv_bfloat16, 128>(p, grid, s);
+  auto by_tokens = [&](auto type, auto size) {
+    using T = decltype(type);
+    constexpr int kDp = decltype(size)::value;
+    return a.max_new > 1 ? step_launch<T, kDp, true>(p, grid, s)
+                         : step_launch<T, kDp, false>(p, grid, s);
+  };
+  auto by_size = [&](auto type) {
+    return dp == 64 ? by_tokens(type, std::integral_constant<int, 64>{})
+                    : by_tokens(type, std::integral_constant<int, 128>{});
+  };
+  return a.dtype == PSPML_DTYPE_F16 ? by_size(__half{})
+                                      : by_size(__nv_bfloat16{});
 }
 
 }  // namespace pspml

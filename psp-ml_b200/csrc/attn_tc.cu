@@ -22,8 +22,10 @@
 //
 // Keys that no row of the CTA sees are not loaded; the values between such a
 // key and the 16-key step of the P V product that holds it are zeroed in
-// shared memory, since 0 * NaN would spread whatever they hold.  Heads of
-// fewer than DP elements are padded with zeros by TMA.
+// shared memory, since 0 * NaN would spread whatever they hold.  Rows that
+// come out non-finite are looked at again (attn_rows.cuh), for what a key
+// that some rows see did to those that do not.  Heads of fewer than DP
+// elements are padded with zeros by TMA.
 //
 // A CTA stays for many items (a pair of tiles and a key head): the next one's
 // loads and first scores run while this one ends.  Many items are handed out
@@ -47,6 +49,7 @@
 #include <type_traits>
 
 #include "attention.h"
+#include "attn_rows.cuh"
 #include "ptx.cuh"
 
 namespace pspml {
@@ -302,7 +305,7 @@ struct TcItem {
   int32_t tokens[2];   // of tile A and B
   int32_t n[2];        // key tiles of A and B in this part
   int32_t j0;          // the part's first key tile
-  int32_t head;
+  int32_t seq, head;
   int32_t pieces;      // CTAs that share the item
   int32_t first_cta;   // of them
   int32_t end;         // no more items
@@ -321,7 +324,7 @@ constexpr uint64_t kItemLimitNs = 5 * kWaitLimitNs;  // longer than any wait wit
 template <typename T, int DP>
 __global__ void __launch_bounds__(kTcThreads, 1)
     k_attn_tc(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
-              const __grid_constant__ CUtensorMap map_v, const TcArgs p) {
+              const __grid_constant__ CUtensorMap map_v, const __grid_constant__ TcArgs p) {
   using Sh = TcShape<DP>;
   extern __shared__ uint8_t smem_raw[];
   __shared__ uint64_t q_full, q_empty, landed, s_full[2], o_done[2], drain;
@@ -509,6 +512,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           d->n[0] = n0;
           d->n[1] = n1;
           d->j0 = j0;
+          d->seq = seq;
           d->head = head;
           d->pieces = pieces;
           d->first_cta = first_cta;
@@ -879,6 +883,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       const bool real = tk < v_item->tokens[t];
       const int64_t out_row = row0 + t * p.tile_tokens + tk;
       const int h = head * p.group + (row - tk * p.group);
+      float check = 0.0f;  // NaN once an output of the row is not finite
       if (ok) {
         const float f = pieces > 1 ? 1.0f : (l == 0.0f ? 0.0f : 1.0f / l);
         const int64_t at = out_row * a.o_token + h * a.o_head;
@@ -898,8 +903,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             if (pieces == 1) {
 #pragma unroll
               for (int x = 0; x < 32; x += 16)
-                if (c * 32 + x < a.dim)
+                if (c * 32 + x < a.dim) {
                   store16<T>(a, at + c * 32 + x, v + x, c * 32 + x + 16 <= a.dim, p.wide_out);
+#pragma unroll
+                  for (int y = 0; y < 16; ++y) check = fmaf(v[x + y], 0.0f, check);
+                }
             } else {
               float4* dst = p.part_o + (slot * (DP / 4) + c * 8) * 256 + t * 128 + row;
 #pragma unroll
@@ -975,14 +983,33 @@ __global__ void __launch_bounds__(kTcThreads, 1)
               for (int y = 0; y < kCols; ++y) acc[y] *= inv;
 #pragma unroll
               for (int y = 0; y < kCols; y += 16)
-                if (col + y < a.dim)
+                if (col + y < a.dim) {
                   store16<T>(a, at + col + y, acc + y, col + y + 16 <= a.dim, p.wide_out);
+#pragma unroll
+                  for (int z = 0; z < 16; ++z) check = fmaf(acc[y + z], 0.0f, check);
+                }
             }
             if (a.lse != nullptr)
               a.lse[orow * a.q_heads + oh] =
                   sum == 0.0f ? -INFINITY : (log2f(sum) + bs) * 0.69314718055994531f;
           }
         }
+      }
+      const uint32_t bad = __ballot_sync(~0u, check != 0.0f);
+      if (bad != 0) {
+        AttnRows r;
+        const int seq = v_item->seq;
+        r.table = a.paged ? a.pages + seq * a.pages_stride : nullptr;
+        r.begin = row0 - v_item->place0;  // of packed keys
+        r.keys = v_item->keys;
+        r.lo = v_item->lo;
+        r.hi = v_item->hi_all;
+        r.row0 = row0 + t * p.tile_tokens;
+        r.place0 = v_item->place0 + t * p.tile_tokens;
+        r.head = head;
+        r.group = p.group;
+        r.first = (warp % 4) * 32;
+        attn_rows_again<T, DP>(a, r, bad);
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&item_empty[it & 1]);

@@ -615,3 +615,98 @@ def test_nothing_to_do(ctx, at):
     at.prompt(ctx, q, q, q, torch.zeros(1, dtype=torch.int32, device="cuda"), out)
     torch.cuda.synchronize()
     assert (out == 5).all()
+
+
+# What a key holds must not reach rows that do not see it, in the tiles of the
+# rows that do: (token from the end, column or None for all, value, in k or v).
+POISON = [(1, 3, NAN, "v"), (9, None, math.inf, "v"), (70, 7, -math.inf, "v"), (71, 7, NAN, "v"),
+          (190, 1, NAN, "v"), (2, None, NAN, "k")]
+
+
+def _check_poisoned(out, lse, want, scale8=None, zero8=0):
+    """Finite where the formula is finite, and to the usual tolerance; not finite where it is
+    not."""
+    o, l, tol_o, tol_l = want
+    fine = torch.isfinite(o)
+    assert not fine.all()
+    if scale8 is None:
+        assert not torch.isfinite(out[~fine]).any()
+    if not fine.any():
+        pass
+    elif scale8 is None:
+        _close(out[fine], o[fine], tol_o[fine], "rows that do not see the bad keys")
+    else:
+        exact = (o[fine] / scale8 + zero8).clamp(-128, 127)
+        _close(out[fine], exact, 0.5 + tol_o[fine] / scale8 + 1e-3, "S8")
+    seen = torch.isnan(l)
+    _close_lse(lse[~seen], l[~seen], tol_l[~seen])
+    assert torch.isnan(lse[seen]).all()
+
+
+def _poison(k, v, column_limit, deepest=1000):
+    for back, column, value, where in POISON:
+        if back <= min(k.shape[0], deepest):
+            x = (k if where == "k" else v)[k.shape[0] - back]
+            x[:, slice(None) if column is None else min(column, column_limit)] = value
+
+
+@pytest.mark.parametrize("tokens,hq,hkv,dim,dtype,causal_window", [
+    (300, 4, 2, 128, BF16, 0), (257, 8, 1, 64, F16, 0), (12, 3, 1, 64, BF16, 0),
+    (700, 6, 2, 80, BF16, 130), (129, 2, 2, 96, F16, 3), (2600, 1, 1, 128, BF16, 0),
+    (1500, 40, 40, 64, F16, 64), (500, 4, 2, 192, BF16, 0)])
+def test_prompt_masked_keys_hold_nan(ctx, at, tokens, hq, hkv, dim, dtype, causal_window):
+    g = _gen(40)
+    q, k, v = (_rand(g, tokens, h, dim, dtype=dtype) for h in (hq, hkv, hkv))
+    _poison(k, v, dim - 1)
+    out, lse = torch.zeros_like(q), torch.zeros((tokens, hq), device="cuda")
+    out8 = torch.zeros((tokens, hq, dim), dtype=torch.int8, device="cuda")
+    at.prompt(ctx, q, k, v, _starts([tokens]), out, lse=lse, window=causal_window)
+    at.prompt(ctx, q, k, v, _starts([tokens]), at.Quantised(out8, 0.02, -3), window=causal_window)
+    ctx.check_device()
+    first = max(0, tokens - 400)          # the rows near the bad keys, and a few before
+    rows = [0] + list(range(max(1, first), tokens)) if tokens > 1 else [0]
+    parts = [ref.attend(q[r:r + 1], k, v, r, True, causal_window, dim ** -0.5) for r in rows]
+    want = [torch.cat(x) for x in zip(*parts)]
+    _check_poisoned(out[rows], lse[rows], want)
+    _check_poisoned(out8[rows], lse[rows], want, 0.02, -3)
+
+
+@pytest.mark.parametrize("bound", [4, 80])
+@pytest.mark.parametrize("deepest", [2, 1000])  # 1000: keys that all rows see as well
+@pytest.mark.parametrize("lengths,new,hq,hkv,dim,page,dtype,window", [
+    ([600, 70], [4, 4], 8, 4, 128, 16, BF16, 0), ([90, 300, 5, 2000], [4, 3, 4, 2], 4, 1, 64, 8, F16, 0),
+    ([3, 40], [4, 2], 2, 1, 80, 16, BF16, 0), ([5000, 1200], [4, 4], 4, 2, 128, 32, F16, 3),
+    ([900], [4], 16, 4, 96, 16, BF16, 200)])
+def test_cached_masked_keys_hold_nan(ctx, at, bound, deepest, lengths, new, hq, hkv, dim, page, dtype,
+                                     window):
+    # Also rows that see no key at all beside rows that do ([3, 40] with 4 new tokens).
+    c = _Paged(_gen(41), lengths, hkv, dim, page, dtype, "slots")
+    for s, n in enumerate(lengths):
+        _poison(c.keys[s], c.values[s], dim - 1, deepest)
+        j = torch.arange(n, device="cuda")
+        ids = c.table[s].long()[j // page]
+        c.k[ids, j % page], c.v[ids, j % page] = c.keys[s], c.values[s]
+    q = _rand(_gen(42), sum(new), hq, dim, dtype=dtype)
+    out, lse = torch.zeros_like(q), torch.zeros((sum(new), hq), device="cuda")
+    at.cached(ctx, q, at.KvCache(c.k, c.v), _starts(new), c.lengths, c.table, out, bound, lse=lse,
+              window=window)
+    ctx.check_device()
+    a, parts = 0, []
+    for s, n in enumerate(new):
+        parts.append(ref.attend(q[a:a + n], c.keys[s], c.values[s], lengths[s] - n, True, window,
+                                dim ** -0.5))
+        a += n
+    want = [torch.cat(x) for x in zip(*parts)]
+    assert deepest > 2 or torch.isfinite(want[0]).any()
+    _check_poisoned(out, lse, want)
+
+
+@pytest.mark.parametrize("dim,hq,hkv", [(128, 8, 2), (64, 3, 3)])
+def test_all_values_nan_or_infinite(ctx, at, dim, hq, hkv):
+    # Every row sees a bad key: nothing is finite, and nothing takes long.
+    q, k = (_rand(_gen(43), 4000, h, dim, dtype=BF16) for h in (hq, hkv))
+    out = torch.zeros_like(q)
+    for value in (NAN, math.inf):
+        at.prompt(ctx, q, k, torch.full_like(k, value), _starts([4000]), out)
+        ctx.check_device()
+        assert not torch.isfinite(out).any()
