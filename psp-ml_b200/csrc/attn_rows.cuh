@@ -6,8 +6,11 @@
 // their outputs (a multiply-add a value) and come here with the rows that are
 // not finite:
 //   1. a token's rows are done again only if a masked key among those that
-//      were multiplied has a non-finite value in a column in which no key
-//      that the token sees has one: else the rows are what the formula gives;
+//      were multiplied has a non-finite value in a column that the keys the
+//      token sees have not settled.  A NaN among them settles a column, and so
+//      do infinities of both signs: whatever the weights, the sum is NaN with
+//      and without the masked keys.  One sign alone does not: the formula
+//      gives that infinity, 0 * v turned it into NaN;
 //   2. eight rows at a time: a lane holds a few columns of all eight, and each
 //      key is read once; a row's score is summed over the lanes and kept by
 //      four of them, and values of keys that a row does not see are skipped.
@@ -17,6 +20,8 @@
 // with token 12127 bad, 3 ms with token 100 or all of them bad, 1.7 ms with
 // none.  Sums and statistics are 32-bit, weights are not rounded.
 #pragma once
+
+#include <cmath>
 
 #include "attention.h"
 
@@ -80,10 +85,11 @@ __device__ __noinline__ void attn_rows_again(const AttnArgs& a, const AttnRows& 
   auto begin_of = [&](int64_t place) {
     return a.window > 0 && place - a.window + 1 > 0 ? place - a.window + 1 : int64_t{0};
   };
-  // The lane's columns in which a key of [j0, j1) is not finite; `stop`: once
-  // all of these have been found.
-  auto bad_columns = [&](int64_t j0, int64_t j1, uint32_t stop) {
-    uint32_t found = 0;
+  // The lane's columns in which keys of [j0, j1) hold a value that is not
+  // finite (`seen` false), or values that make any weighted sum NaN (`seen`
+  // true); over once all columns of `stop` have been found.
+  auto bad_columns = [&](int64_t j0, int64_t j1, bool seen, uint32_t stop) {
+    uint32_t nan = 0, above = 0, below = 0, found = 0;
     for (int64_t j = j1; j > j0; j -= kScan) {
       Columns c[kScan];
 #pragma unroll
@@ -95,8 +101,13 @@ __device__ __noinline__ void attn_rows_again(const AttnArgs& a, const AttnRows& 
 #pragma unroll
       for (int b = 0; b < kScan; ++b)
 #pragma unroll
-        for (int x = 0; x < C; ++x)
-          found |= isfinite(to_f32(c[b].x[x])) ? 0u : 1u << x;
+        for (int x = 0; x < C; ++x) {
+          const float f = to_f32(c[b].x[x]);
+          nan |= f != f ? 1u << x : 0u;
+          above |= f == INFINITY ? 1u << x : 0u;
+          below |= f == -INFINITY ? 1u << x : 0u;
+        }
+      found = nan | (seen ? above & below : above | below);
       if (!__any_sync(~0u, stop & ~found)) break;
     }
     return found;
@@ -111,10 +122,10 @@ __device__ __noinline__ void attn_rows_again(const AttnArgs& a, const AttnRows& 
       last = tok;
       const int64_t beg = begin_of(r.place0 + tok), end = end_of(r.place0 + tok);
       const bool empty = end <= beg;
-      uint32_t masked = bad_columns(r.lo, empty || beg > r.hi ? r.hi : beg, ~0u);
+      uint32_t masked = bad_columns(r.lo, empty || beg > r.hi ? r.hi : beg, false, ~0u);
       if (!empty) {
-        masked |= bad_columns(end > r.lo ? end : r.lo, r.hi, ~0u);
-        if (__any_sync(~0u, masked)) masked &= ~bad_columns(beg, end, masked);
+        masked |= bad_columns(end > r.lo ? end : r.lo, r.hi, false, ~0u);
+        if (__any_sync(~0u, masked)) masked &= ~bad_columns(beg, end, true, masked);
       }
       token_again = __any_sync(~0u, masked);
     }
