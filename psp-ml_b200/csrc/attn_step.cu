@@ -121,7 +121,8 @@ __device__ __forceinline__ float ex2(float x) {
 
 // Tiles of one sequence and key head, and where its keys begin and end.
 struct StepSeq {
-  int64_t begin, keys, rows;  // rows: at most max_new
+  int64_t begin, rows;        // rows: at most max_new
+  int64_t keys;               // one past the last key that any of these rows sees
   int64_t place0;             // position of row 0
   int64_t lo;                 // first key any row sees
   int64_t first_tile;
@@ -131,9 +132,12 @@ __device__ __forceinline__ StepSeq step_seq(const StepArgs& p, int s) {
   const SeqSpan sp = seq_span(p.a, s);
   StepSeq r;
   r.begin = sp.begin;
-  r.keys = sp.keys;
   r.place0 = sp.keys - sp.rows;
   r.rows = sp.rows < p.a.max_new ? sp.rows : p.a.max_new;
+  // The keys of rows past max_new are not seen, so they are not multiplied
+  // either: a single row (kMulti false) relies on it.
+  const int64_t seen = r.place0 + r.rows;
+  r.keys = !p.a.causal || seen > sp.keys ? sp.keys : (seen < 0 ? 0 : seen);
   r.lo = 0;
   if (p.a.window > 0 && r.place0 - p.a.window + 1 > 0) r.lo = r.place0 - p.a.window + 1;
   r.first_tile = r.lo / kStepTile;

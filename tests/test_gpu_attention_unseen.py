@@ -130,3 +130,31 @@ def test_cached_seen_infinities(ctx, at, mix, bound, lengths, new, hq, hkv, dim,
         parts.append(_wants(q[a:a + m], keys[s], values[s], lengths[s] - m, range(m)))
         a += m
     _same(out, lse, tuple(torch.cat(x) for x in zip(*parts)))
+
+
+@pytest.mark.parametrize("window", [0, 37])
+@pytest.mark.parametrize("computed", [1, 2, 40])  # rows of each sequence that the call computes
+@pytest.mark.parametrize("lengths,new,hq,hkv,dim,dtype", [
+    ([130, 700, 3], [3, 60, 3], 8, 2, 128, BF16), ([50], [50], 4, 1, 64, F16),
+    ([64, 2000, 1], [64, 45, 1], 4, 2, 80, BF16)])
+def test_rows_past_max_new_hold_nan(ctx, at, window, computed, lengths, new, hq, hkv, dim, dtype):
+    # Keys of the rows that are not computed hold NaN and infinities; those rows stay as they are.
+    keys = [_rand(20 + s, n, hkv, dim, dtype=dtype) for s, n in enumerate(lengths)]
+    values = [_rand(24 + s, n, hkv, dim, dtype=dtype) for s, n in enumerate(lengths)]
+    done = [min(m, computed) for m in new]
+    for k, v, n, m, d in zip(keys, values, lengths, new, done):
+        if d < m:
+            v[n - m + d:] = NAN
+            v[n - 1] = INF
+            k[n - m + d:, :, 1] = NAN
+    cache, n, table = _cache(at, keys, values, 16)
+    q = _rand(28, sum(new), hq, dim, dtype=dtype)
+    out, lse = torch.full_like(q, 7.0), torch.full((sum(new), hq), 7.0, device="cuda")
+    at.cached(ctx, q, cache, _starts(new), n, table, out, computed, lse=lse, window=window)
+    ctx.check_device()
+    a = 0
+    for s, (m, d) in enumerate(zip(new, done)):
+        _same(out[a:a + d], lse[a:a + d],
+              _wants(q[a:a + d], keys[s], values[s], lengths[s] - m, range(d), window))
+        assert (out[a + d:a + m] == 7).all() and (lse[a + d:a + m] == 7).all()
+        a += m
