@@ -323,10 +323,11 @@ int pspml_forward_timed(pspml_model* m, const int8_t* dev_in, int8_t* dev_out,
  *
  * The first pspml_attention_* call of a context allocates about 40 MB for
  * the pieces of calls that are split over the device; make it before any
- * stream capture.  Later calls allocate nothing.  Calls of one context on
- * different streams share that memory and are ordered after one another by
- * the library; under capture the order is the caller's: replays of graphs
- * that share a context run one at a time. */
+ * stream capture.  Later calls allocate nothing.  Calls of one context share
+ * that memory and are ordered after one another by the library, whatever
+ * streams they are given; the host makes them one at a time.  Under capture
+ * the order is the caller's: a replay of a graph with such calls runs neither
+ * beside another replay of the same context nor beside a direct call. */
 typedef enum pspml_dtype {
   PSPML_DTYPE_F32 = 0,
   PSPML_DTYPE_F16 = 1,

@@ -251,9 +251,12 @@ bool vector_form(const AttnArgs& a) {
           a.o_token | a.o_head) % 8 == 0;
 }
 
-// Split calls of one context run one after another even when they are given
-// different streams, since they share its workspace.  Under capture an event
-// of the outside cannot be waited for: there the caller keeps the order.
+// Split calls of one context run one after another whatever streams they are
+// given, since they share its workspace.  Every call waits for the last one's
+// event, also on an equal handle, which need not be the same stream: each host
+// thread has a default stream of its own under one handle, and a destroyed
+// stream's handle may come back while its work runs.  Under capture an event of
+// the outside cannot be waited for: there the caller keeps the order.
 int with_workspace(pspml_ctx* ctx, const AttnArgs& a, cudaStream_t s,
                    cudaError_t (*launch)(const AttnArgs&, const AttnWork&, cudaStream_t)) {
   cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
@@ -273,14 +276,13 @@ int with_workspace(pspml_ctx* ctx, const AttnArgs& a, cudaStream_t s,
   w.counters = ctx->dev_err + 64;
   w.err = ctx->dev_err;
   w.num_sms = ctx->num_sms;
-  if (order && ctx->attn_used && ctx->attn_stream != s &&
+  if (order && ctx->attn_used &&
       (st = cuda_status(cudaStreamWaitEvent(s, ctx->attn_done, 0), "cudaStreamWaitEvent")))
     return st;
   if ((st = cuda_status(launch(a, w, s), "attention launch"))) return st;
   if (order) {
     if ((st = cuda_status(cudaEventRecord(ctx->attn_done, s), "cudaEventRecord"))) return st;
     ctx->attn_used = true;
-    ctx->attn_stream = s;
   }
   return PSPML_OK;
 }

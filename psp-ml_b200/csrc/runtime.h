@@ -25,10 +25,9 @@ struct pspml_ctx {
   size_t workspace_bytes = 0;
   cudaStream_t stream = nullptr;    // internal stream for synchronous work
   // Pieces of split attention calls, allocated by the first such call, and
-  // the last call that used them: one on another stream waits for it.
+  // the end of the last call that used them, for which the next one waits.
   uint8_t* attn_workspace = nullptr;
   cudaEvent_t attn_done = nullptr;
-  cudaStream_t attn_stream = nullptr;
   bool attn_used = false;
 };
 
