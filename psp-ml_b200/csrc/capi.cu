@@ -276,7 +276,11 @@ int pspml_ctx_check_device(pspml_ctx* ctx) {
                        "read device error word");
   if (st) return st;
   if (v != 0) {
-    // The counters too: a kernel that gave up may have left one part-way.
+    // The counters too: a kernel that gave up may have left one part-way.  Not
+    // before everything on the device has ended, on streams that the context's
+    // own is not ordered with too: an attention call still counts on them.
+    st = cuda_status(cudaDeviceSynchronize(), "wait before clearing the error word");
+    if (st) return st;
     cudaMemsetAsync(ctx->dev_err, 0, kDevErrBytes, ctx->stream);
     cudaStreamSynchronize(ctx->stream);
     char buf[96];

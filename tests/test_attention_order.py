@@ -73,3 +73,16 @@ def test_calls_wait_for_the_last_one(fake, context, streams, max_new, kernel):
         _cached(fake, context, s, max_new)
     a, b = streams
     assert _log(fake) == [(kernel, a), ("record", a), ("wait", b), (kernel, b), ("record", b)]
+
+
+def test_counters_are_cleared_when_nothing_runs(fake, context):
+    # A call made after a kernel gave up may still run on a stream that the clearing does not wait
+    # for, and counts on the counters.
+    assert fake.pspml_ctx_wait_selftest(context, 1, 0) == capi.OK
+    _cached(fake, context, 7)
+    fake.fake_clear()
+    assert fake.pspml_ctx_check_device(context) == capi.ERR_DEVICE_WAIT
+    whats = [what for what, _ in _log(fake)]
+    assert "memset" in whats
+    assert "synchronize device" in whats[:whats.index("memset")]
+    assert fake.pspml_ctx_check_device(context) == capi.OK
