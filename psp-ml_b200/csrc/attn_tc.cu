@@ -49,6 +49,7 @@
 #include <type_traits>
 
 #include "attention.h"
+#include "attn_giveup.cuh"
 #include "attn_rows.cuh"
 #include "ptx.cuh"
 
@@ -134,13 +135,13 @@ __device__ __forceinline__ void tc_fail(unsigned* err, volatile int* abort, unsi
 // at a hardware barrier: polls of an mbarrier would take issue slots from the
 // two softmax warps on the MMA warp's scheduler, which set the pace (2121 us
 // against 1854 at 16384 tokens and 32 heads with tight and with rare polls).
-// Both sides walk all their key tiles whatever happens, so neither waits for
-// an arrival that does not come.
-__device__ __forceinline__ void prob_arrive(int t, int h) {
-  asm volatile("bar.arrive %0, 160;" ::"r"(2 + t * kPieces + h) : "memory");
+// These waits have no limit; attn_giveup.cuh says why they end.  `n`: key tiles
+// of tile t before this one.
+__device__ __forceinline__ void prob_arrive(int t, int h, uint32_t n) {
+  asm volatile("bar.arrive %0, 160;" ::"r"(prob_barrier(t, h, n)) : "memory");
 }
-__device__ __forceinline__ void prob_wait(int t, int h) {
-  asm volatile("bar.sync %0, 160;" ::"r"(2 + t * kPieces + h) : "memory");
+__device__ __forceinline__ void prob_meet(int t, int h, uint32_t n) {
+  asm volatile("bar.sync %0, 160;" ::"r"(prob_barrier(t, h, n)) : "memory");
 }
 
 // Eight neighbouring outputs of a row.
@@ -320,6 +321,7 @@ struct TcShare {
   SeqSpan span{0, 0, 0};
 };
 constexpr uint64_t kItemLimitNs = 5 * kWaitLimitNs;  // longer than any wait within an item
+static_assert(kPieces == 2, "prob_barrier's layout");
 
 template <typename T, int DP>
 __global__ void __launch_bounds__(kTcThreads, 1)
@@ -333,6 +335,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   __shared__ TcItem items[2];
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_word;
+  __shared__ int book;  // of items (attn_giveup.cuh)
   __shared__ int s_last, s_longest, s_scan[kTcThreads / 32];
   const AttnArgs& a = p.a;
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
@@ -343,6 +346,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 
   if (tid == 0) {
     abort_word = 0;
+    book = 0;
     s_longest = 0;
     mbar_init(&q_full, 1);
     mbar_init(&q_empty, 1);
@@ -430,15 +434,19 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
-  // Item `it` of this CTA, published by warp 8.  Whoever has taken an item
-  // walks all of it, and every warp takes the same items: this wait does not
-  // look at the abort flag.
+  // Item `it` of this CTA, published by warp 8.  Every warp takes the same
+  // items, and whoever has taken one walks all of it.
   auto take = [&](int it) -> const TcItem* {
-    const bool got =
-        __all_sync(~0u, mbar_wait(&item_full[it & 1], static_cast<uint32_t>((it >> 1) & 1),
-                                  nullptr, kItemLimitNs));
-    if (!got && lane == 0) tc_fail(p.err, abort, kDevErrEpiWait);
-    return got ? &items[it & 1] : nullptr;
+    if (!__all_sync(~0u, mbar_wait(&item_full[it & 1], static_cast<uint32_t>((it >> 1) & 1), abort,
+                                   kItemLimitNs))) {
+      bool closed = false;
+      if (lane == 0) {
+        closed = item_close(&book, it);
+        if (closed) tc_fail(p.err, abort, kDevErrEpiWait);
+      }
+      if (__any_sync(~0u, closed)) return nullptr;
+    }
+    return &items[it & 1];
   };
   // Keys of tile j that some row sees: [v_lo, v_hi) of its 128.
   auto v_lo = [](int64_t lo, int64_t start, int j) {
@@ -466,22 +474,24 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       for (int it = 0;; ++it) {
         TcItem* const d = &items[it & 1];
         if (it >= 2 && !mbar_wait(&item_empty[it & 1], static_cast<uint32_t>(((it >> 1) - 1) & 1),
-                                  nullptr, kItemLimitNs)) {
+                                  abort, kItemLimitNs)) {
           tc_fail(p.err, abort, kDevErrTmaWait);
           ok = false;
         }
-        bool have = __all_sync(~0u, ok && !*abort);
-        if (cut) {
-          have = have && at < share.stop;
-        } else {
+        if (!__all_sync(~0u, ok && !*abort)) {
+          // The record may still be that of an item that some warp has not taken.
+          if (lane == 0) item_close(&book, it);
+          break;
+        }
+        bool have = at < share.stop;
+        if (!cut) {
           head = static_cast<int>(next % a.kv_heads);
-          have = have && next < p.items &&
-                 tc_locate(p, next / a.kv_heads, lane, &seq, &pair, &span);
+          have = next < p.items && tc_locate(p, next / a.kv_heads, lane, &seq, &pair, &span);
         }
         if (!have) {
           if (lane == 0) {
             d->end = 1;
-            mbar_arrive(&item_full[it & 1]);
+            if (item_publish(&book, it)) mbar_arrive(&item_full[it & 1]);
           }
           break;
         }
@@ -517,9 +527,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           d->pieces = pieces;
           d->first_cta = first_cta;
           d->end = 0;
-          mbar_arrive(&item_full[it & 1]);
+          ok = item_publish(&book, it);
+          if (ok) mbar_arrive(&item_full[it & 1]);
         }
-        __syncwarp();
+        if (!__all_sync(~0u, ok)) break;
         // The next item: asked for now, looked at when this one's loads are out.
         unsigned taken = 0;
         if (more && lane == 0) taken = atomicAdd(p.next, 1u);
@@ -623,7 +634,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             }
         }
       }
-      if (__any_sync(~0u, *abort)) {  // the copies in flight land before the CTA leaves
+      if (__any_sync(~0u, !ok || *abort)) {  // the copies in flight land before the CTA leaves
         if (q_loads > 0) mbar_wait(&q_full, static_cast<uint32_t>((q_loads - 1) & 1), nullptr);
         if (landings > 0) mbar_wait(&landed, static_cast<uint32_t>((landings - 1) & 1), nullptr);
         for (int i = issued > Sh::kSlots ? issued - Sh::kSlots : 0; i < issued; ++i)
@@ -668,10 +679,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         };
         // P comes in pieces: the product of one runs while the next one's
         // weights are found.
+        uint32_t done[2] = {0, 0};   // key tiles of A and of B so far
         auto pv = [&](int t, int i, int slot, int k0, int k1, uint64_t* freed) {
 #pragma unroll
           for (int h = 0; h < kPieces; ++h) {
-            prob_wait(t, h);
+            prob_meet(t, h, done[t] + static_cast<uint32_t>(i));
             tc_fence_after();
             if (elect_one()) {
               const uint64_t b = make_sdesc(kv_addr + slot * Sh::kTileBytes, 16384, 1024, 2);
@@ -688,7 +700,6 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             __syncwarp();
           }
         };
-        uint32_t done[2] = {0, 0};   // key tiles of A and of B so far
         int k_slot = 0, q_items = 0; // ring slot and phase of the next key tile
         uint32_t k_phase = 0;
         for (int it = 0;; ++it) {
@@ -764,6 +775,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     const uint32_t lanes = static_cast<uint32_t>((warp % 4) * 32) << 16;
     const uint32_t ts = tmem + Sh::kS + t * 128 + lanes, to = tmem + Sh::kO + t * DP + lanes;
     uint32_t done = 0;  // key tiles so far
+    bool ok = true;     // until one of this warp's waits has failed
     for (int it = 0;; ++it) {
       const TcItem* const d = take(it);
       if (d == nullptr || d->end) break;
@@ -789,14 +801,19 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         all_beg = beg_of(place + d->tokens[t] - 1);
       }
       float m = -INFINITY, l = 0.0f;
-      bool ok = true;
       for (int i = 0; i < nt; ++i) {
         const int kb = i * kKeys;
-        if (!mbar_wait(&s_full[t], (done + static_cast<uint32_t>(i)) & 1u, abort)) {
+        const uint32_t n = done + static_cast<uint32_t>(i);
+        if (ok && !mbar_wait(&s_full[t], n & 1u, abort)) {
           tc_fail(p.err, abort, kDevErrEpiWait);
           ok = false;
         }
-        __syncwarp();
+        ok = __all_sync(~0u, ok);
+        if (!ok) {
+#pragma unroll
+          for (int h = 0; h < kPieces; ++h) prob_meet(t, h, n);
+          continue;
+        }
         tc_fence_after();
         uint32_t s[kKeys];
         tmem_ld128(ts, s);
@@ -857,7 +874,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
           if ((c + 1) % (4 / kPieces) == 0) {
             tmem_wait_st();
             tc_fence_before();
-            prob_arrive(t, c / (4 / kPieces));
+            prob_arrive(t, c / (4 / kPieces), n);
           }
         }
         float sa, sb, sc, sd;
