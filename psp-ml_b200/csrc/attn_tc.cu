@@ -126,9 +126,37 @@ __device__ __forceinline__ uint64_t f2_add(uint64_t a, uint64_t b) {
   return r;
 }
 
-__device__ __forceinline__ void tc_fail(unsigned* err, volatile int* abort, unsigned code) {
-  *abort = 1;
+// The CTA's state: kGaveUp once a wait has run out, and kRowsAgain for every
+// warp that is doing rows again.
+constexpr int kGaveUp = 1;
+constexpr int kRowsAgain = 2;
+__device__ __forceinline__ void tc_fail(unsigned* err, int* state, unsigned code) {
+  atomicOr(state, kGaveUp);
   atomicCAS(err, 0u, code);
+}
+// The waits of ptx.cuh (kPoll: without the suspend-time hint), which end when
+// the CTA has given up.  Rows done again hold the CTA's other warps up for as
+// long as their keys take, seconds for a long context: no signal is lost, and
+// the limit does not run meanwhile.
+template <bool kPoll = false>
+__device__ __forceinline__ bool tc_wait(uint64_t* bar, uint32_t parity, const int* state,
+                                        uint64_t limit_ns = kWaitLimitNs) {
+  auto passed = [&]() {
+    return kPoll ? mbar_try_wait_poll(bar, parity) : mbar_try_wait(bar, parity);
+  };
+  if (passed()) return true;
+  uint64_t t0 = global_timer_ns();
+  while (true) {
+#pragma unroll 1
+    for (int i = 0; i < (kPoll ? 64 : 32); ++i)
+      if (passed()) return true;
+    const int now = *static_cast<const volatile int*>(state);
+    if (now != 0) {
+      if (now & kGaveUp) return false;
+      t0 = global_timer_ns();
+    }
+    if (global_timer_ns() - t0 > limit_ns) return false;
+  }
 }
 
 // Piece h of tile t's P is handed from its four softmax warps to the MMA warp
@@ -320,7 +348,9 @@ struct TcShare {
   int64_t pair = 0;
   SeqSpan span{0, 0, 0};
 };
-constexpr uint64_t kItemLimitNs = 5 * kWaitLimitNs;  // longer than any wait within an item
+// Of the wait for the next item, and of the loader's for a record: longer than
+// any wait within an item, of which the others wait for several.
+constexpr uint64_t kItemLimitNs = 5 * kWaitLimitNs;
 static_assert(kPieces == 2, "prob_barrier's layout");
 
 template <typename T, int DP>
@@ -334,18 +364,19 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   __shared__ uint64_t item_full[2], item_empty[2];
   __shared__ TcItem items[2];
   __shared__ uint32_t tmem_slot;
-  __shared__ int abort_word;
+  __shared__ int state_word;
   __shared__ int book;  // of items (attn_giveup.cuh)
   __shared__ int s_last, s_longest, s_scan[kTcThreads / 32];
   const AttnArgs& a = p.a;
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
-  volatile int* abort = &abort_word;
+  int* const state = &state_word;
+  auto gave_up = [&]() { return (*static_cast<volatile int*>(state) & kGaveUp) != 0; };
   uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
   uint8_t* sq = smem;
   uint8_t* slots = smem + 2 * Sh::kTileBytes;
 
   if (tid == 0) {
-    abort_word = 0;
+    state_word = 0;
     book = 0;
     s_longest = 0;
     mbar_init(&q_full, 1);
@@ -437,12 +468,12 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   // Item `it` of this CTA, published by warp 8.  Every warp takes the same
   // items, and whoever has taken one walks all of it.
   auto take = [&](int it) -> const TcItem* {
-    if (!__all_sync(~0u, mbar_wait(&item_full[it & 1], static_cast<uint32_t>((it >> 1) & 1), abort,
-                                   kItemLimitNs))) {
+    if (!__all_sync(~0u, tc_wait(&item_full[it & 1], static_cast<uint32_t>((it >> 1) & 1), state,
+                                 kItemLimitNs))) {
       bool closed = false;
       if (lane == 0) {
         closed = item_close(&book, it);
-        if (closed) tc_fail(p.err, abort, kDevErrEpiWait);
+        if (closed) tc_fail(p.err, state, kDevErrEpiWait);
       }
       if (__any_sync(~0u, closed)) return nullptr;
     }
@@ -473,12 +504,12 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       SeqSpan span = share.span;
       for (int it = 0;; ++it) {
         TcItem* const d = &items[it & 1];
-        if (it >= 2 && !mbar_wait(&item_empty[it & 1], static_cast<uint32_t>(((it >> 1) - 1) & 1),
-                                  abort, kItemLimitNs)) {
-          tc_fail(p.err, abort, kDevErrTmaWait);
+        if (it >= 2 && !tc_wait(&item_empty[it & 1], static_cast<uint32_t>(((it >> 1) - 1) & 1),
+                                state, kItemLimitNs)) {
+          tc_fail(p.err, state, kDevErrTmaWait);
           ok = false;
         }
-        if (!__all_sync(~0u, ok && !*abort)) {
+        if (!__all_sync(~0u, ok && !gave_up())) {
           // The record may still be that of an item that some warp has not taken.
           if (lane == 0) item_close(&book, it);
           break;
@@ -544,8 +575,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         int page = n > 0 ? page_of(j0) : -1;
         if (n > 0) {
           const uint32_t q_phase = static_cast<uint32_t>((q_loads - 1) & 1);
-          if (q_loads > 0 && !mbar_wait(&q_empty, q_phase, abort)) {
-            tc_fail(p.err, abort, kDevErrTmaWait);
+          if (q_loads > 0 && !tc_wait(&q_empty, q_phase, state)) {
+            tc_fail(p.err, state, kDevErrTmaWait);
             ok = false;
           }
           __syncwarp();
@@ -575,8 +606,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                                      : static_cast<int32_t>(span.begin + kb + first);
           const int32_t c3 = a.paged ? page : 0;
           for (int which = 0; which < 2; ++which) {
-            const bool got = mbar_wait(&kv_empty[slot], phase ^ 1u, abort);
-            if (!got) tc_fail(p.err, abort, kDevErrTmaWait);
+            const bool got = tc_wait(&kv_empty[slot], phase ^ 1u, state);
+            if (!got) tc_fail(p.err, state, kDevErrTmaWait);
             if (!__all_sync(~0u, got)) {
               ok = false;
               break;
@@ -592,8 +623,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                             head, c2, c3);
             __syncwarp();
             if (mend) {
-              if (!mbar_wait(&landed, static_cast<uint32_t>(landings & 1), abort)) {
-                tc_fail(p.err, abort, kDevErrTmaWait);
+              if (!tc_wait(&landed, static_cast<uint32_t>(landings & 1), state)) {
+                tc_fail(p.err, state, kDevErrTmaWait);
                 ok = false;
               }
               ++landings;
@@ -634,7 +665,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             }
         }
       }
-      if (__any_sync(~0u, !ok || *abort)) {  // the copies in flight land before the CTA leaves
+      if (__any_sync(~0u, !ok || gave_up())) {  // the copies in flight land before the CTA leaves
         if (q_loads > 0) mbar_wait(&q_full, static_cast<uint32_t>((q_loads - 1) & 1), nullptr);
         if (landings > 0) mbar_wait(&landed, static_cast<uint32_t>((landings - 1) & 1), nullptr);
         for (int i = issued > Sh::kSlots ? issued - Sh::kSlots : 0; i < issued; ++i)
@@ -652,10 +683,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         const uint32_t id_qk = make_idesc_f16(128, kKeys, kFmt, 0);
         const uint32_t id_pv = make_idesc_f16(128, k_steps * 16, kFmt, 1);
         const uint32_t q_addr = smem_u32(sq), kv_addr = smem_u32(slots);
-        // A wait that gives up only raises the abort flag, after which every
+        // A wait that gives up only changes the state, after which every
         // other wait ends at once.
         auto wait = [&](uint64_t* bar, uint32_t phase) {
-          if (!mbar_wait_poll(bar, phase, abort)) tc_fail(p.err, abort, kDevErrMmaWait);
+          if (!tc_wait<true>(bar, phase, state)) tc_fail(p.err, state, kDevErrMmaWait);
           __syncwarp();
         };
         // Descriptors are built once a tile; a step adds its 16-byte units to
@@ -804,8 +835,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       for (int i = 0; i < nt; ++i) {
         const int kb = i * kKeys;
         const uint32_t n = done + static_cast<uint32_t>(i);
-        if (ok && !mbar_wait(&s_full[t], n & 1u, abort)) {
-          tc_fail(p.err, abort, kDevErrEpiWait);
+        if (ok && !tc_wait(&s_full[t], n & 1u, state)) {
+          tc_fail(p.err, state, kDevErrEpiWait);
           ok = false;
         }
         ok = __all_sync(~0u, ok);
@@ -884,8 +915,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       }
       done += static_cast<uint32_t>(nt);
       if (nt > 0 && ok) {
-        ok = mbar_wait(&o_done[t], (done - 1) & 1u, abort);
-        if (!ok) tc_fail(p.err, abort, kDevErrEpiWait);
+        ok = tc_wait(&o_done[t], (done - 1) & 1u, state);
+        if (!ok) tc_fail(p.err, state, kDevErrEpiWait);
         __syncwarp();
         tc_fence_after();
       }
@@ -1026,7 +1057,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         r.head = head;
         r.group = p.group;
         r.first = (warp % 4) * 32;
+        if (lane == 0) atomicAdd(state, kRowsAgain);
         attn_rows_again<T, DP>(a, r, bad);
+        __syncwarp();
+        if (lane == 0) atomicAdd(state, -kRowsAgain);
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&item_empty[it & 1]);

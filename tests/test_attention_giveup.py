@@ -6,7 +6,9 @@ a limit, and the hardware barriers, which have none.  Any limited wait may run
 out at any time, copies and products may never complete, and whatever happens
 every role has to come to its end, with no hardware barrier arrived at twice by
 a warp in one generation.  The barriers' numbers are the kernel's own, from
-csrc/attn_giveup.cuh.  Planted mistakes are found.
+csrc/attn_giveup.cuh.  Planted mistakes are found.  With a clock, waits run out
+by their limit alone, and rows done again (csrc/attn_rows.cuh) that take longer
+than any limit make none of them run out.
 """
 import ctypes
 import random
@@ -68,10 +70,14 @@ class Kernel:
 
     SLOTS = 5
 
-    def __init__(self, items, rng, barrier_of, chance, lost, after="meet", common=True):
+    def __init__(self, items, rng, barrier_of, chance, lost, after="meet", common=True, limit=None,
+                 again=0.0, again_time=0, pause=True):
         self.items, self.rng, self.barrier_of, self.chance, self.lost = (items, rng, barrier_of,
                                                                          chance, lost)
         self.after, self.common = after, common
+        # Steps of the clock: a wait's limit, and rows done again at an item's end.
+        self.limit, self.again, self.again_time, self.pause = limit, again, again_time, pause
+        self.clock = self.busy = 0
         self.abort = False
         self.book = 0
         self.record = [None, None]
@@ -221,6 +227,11 @@ class Kernel:
             if item[2]:
                 yield self.meet(self.group, who)
                 yield self.meet(self.group, who)
+            if self.rng.random() < self.again:
+                self.busy += 1
+                until = self.clock + self.again_time
+                yield (lambda: self.clock >= until), False
+                self.busy -= 1
             self.item_empty[it % 2].arrive()
             it += 1
         yield self.meet(self.block, who)
@@ -237,18 +248,21 @@ class Kernel:
         return True
 
     def run(self):
-        waits, slow = {}, {}
+        waits, slow, since = {}, {}, {}
         for r in [self.loader(), self.mma()] + [self.softmax(t, w) for t in range(2)
                                                 for w in range(4)]:
-            waits[r] = next(r)
+            waits[r], since[r] = next(r), 0
             slow[r] = self.rng.choice([1, 1, 5, 25])
 
         def step(r, answer):
             try:
-                waits[r] = r.send(answer)
+                waits[r], since[r] = r.send(answer), self.clock
             except StopIteration:
                 del waits[r]
         while waits:
+            self.clock += 1
+            if self.busy and self.pause:
+                since = dict.fromkeys(since, self.clock)
             roles = list(waits)
             r = self.rng.choices(roles, [slow[x] for x in roles])[0]
             passed, limited = waits[r]
@@ -256,7 +270,12 @@ class Kernel:
                 step(r, True)
             elif limited and (self.abort or self.rng.random() < self.chance):
                 step(r, False)
+            elif limited and self.limit is not None and self.clock - since[r] > self.limit:
+                step(r, False)
             elif not self.complete() and not any(p() for p, _ in waits.values()):
+                if self.busy:  # nothing else to do meanwhile
+                    self.clock += self.again_time // 20
+                    continue
                 late = [x for x in waits if waits[x][1]]  # nothing will come: limits run out
                 if not late:
                     raise Broken("roles wait without a limit for what does not come")
@@ -319,3 +338,15 @@ def test_barriers_are_the_hardwares_and_apart(barrier_of):
     assert len(set(ids)) == 8 and min(ids) >= 2 and max(ids) < 16
     assert all(barrier_of(t, h, n) == barrier_of(t, h, n + 2)
                for t in range(2) for h in range(PIECES) for n in range(2))
+
+
+@pytest.mark.parametrize("pause", [True, False])
+def test_rows_done_again_outlast_the_limits(barrier_of, pause):
+    gave_up = 0
+    for seed in range(30):
+        rng = random.Random(seed)
+        k = Kernel(_items(rng), rng, barrier_of, 0.0, 0.0, limit=400000, again=0.1,
+                   again_time=2000000, pause=pause)
+        k.run()
+        gave_up += k.abort
+    assert gave_up == 0 if pause else gave_up > 0

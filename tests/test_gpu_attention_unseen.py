@@ -158,3 +158,28 @@ def test_rows_past_max_new_hold_nan(ctx, at, window, computed, lengths, new, hq,
               _wants(q[a:a + d], keys[s], values[s], lengths[s] - m, range(d), window))
         assert (out[a + d:a + m] == 7).all() and (lse[a + d:a + m] == 7).all()
         a += m
+
+
+def test_rows_done_again_outlast_the_wait_limit(ctx, at):
+    # One bad value after a million keys: its tile's rows are done again for longer than the 4 s
+    # that any wait in the kernel may take, while other items wait in the same CTA.
+    keys, seqs, new, dim, page = 1000040, 300, 20, 8, 512
+    need = (keys + page - 1) // page
+    g = torch.Generator(device="cuda").manual_seed(30)
+    pool = torch.randn((2, need + 1, page, 1, dim), generator=g, device="cuda").to(F16)
+    # The sequences share their pages but for the last one of the first sequence.
+    table = torch.arange(need, dtype=torch.int32, device="cuda")[None].repeat(seqs, 1)
+    pool[:, need] = pool[:, need - 1]
+    table[0, -1] = need
+    pool[1, need, (keys - 2) % page, 0, 3] = NAN
+    q = _rand(31, seqs * new, 1, dim, dtype=F16, size=0.1)
+    out, lse = torch.zeros_like(q), torch.zeros((seqs * new, 1), device="cuda")
+    lengths = torch.full((seqs,), keys, dtype=torch.int32, device="cuda")
+    at.cached(ctx, q, at.KvCache(pool[0], pool[1]), _starts([new] * seqs), lengths, table, out, new,
+              lse=lse)
+    ctx.check_device()
+    for s in (0, 1, 147, 148, 149, 150, 151, 298, 299):
+        k, v = (pool[i][table[s].long()].view(-1, 1, dim)[:keys] for i in range(2))
+        rows = slice(s * new, (s + 1) * new)
+        _same(out[rows], lse[rows], _wants(q[rows], k, v, keys - new, range(new)))
+    assert torch.isfinite(out[new:]).all()
