@@ -1058,6 +1058,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         r.group = p.group;
         r.first = (warp % 4) * 32;
         if (lane == 0) atomicAdd(state, kRowsAgain);
+        __syncwarp();  // other lanes write these rows again: after this lane's stores
         attn_rows_again<T, DP>(a, r, bad);
         __syncwarp();
         if (lane == 0) atomicAdd(state, -kRowsAgain);

@@ -160,6 +160,24 @@ def test_rows_past_max_new_hold_nan(ctx, at, window, computed, lengths, new, hq,
         a += m
 
 
+@pytest.mark.parametrize("tokens,hq,hkv,dim,dtype", [(700, 8, 2, 128, BF16), (2600, 1, 1, 64, F16)])
+def test_rows_done_again_stay(ctx, at, tokens, hq, hkv, dim, dtype):
+    # Other lanes of the warp write a row done again than wrote it first: every time the second
+    # writing is the one that stays.  2600 tokens of one head are cut over the device.
+    q, k, v = (_rand(32 + i, tokens, h, dim, dtype=dtype) for i, h in enumerate((hq, hkv, hkv)))
+    v[::50, :, 1] = NAN
+    v[:100] = v[:100].nan_to_num()
+    out, lse = torch.zeros_like(q), torch.zeros((tokens, hq), device="cuda")
+    at.prompt(ctx, q, k, v, _starts([tokens]), out, lse=lse)
+    rows = list(range(0, tokens, 13))
+    _same(out[rows], lse[rows], _wants(q, k, v, 0, rows))
+    again = torch.empty_like(out)
+    for _ in range(30):
+        at.prompt(ctx, q, k, v, _starts([tokens]), again.fill_(7))
+        assert torch.equal(again.isnan(), out.isnan())
+        assert torch.equal(again.nan_to_num(), out.nan_to_num())
+
+
 def test_rows_done_again_outlast_the_wait_limit(ctx, at):
     # One bad value after a million keys: its tile's rows are done again for longer than the 4 s
     # that any wait in the kernel may take, while other items wait in the same CTA.
