@@ -5,7 +5,7 @@ describes its tensors to the C ABI and makes one call.  Heads are tensors
 [tokens][heads][dim] whose last dimension is contiguous (slices of one
 projection's output are fine); index tensors are contiguous.  Everything is
 asynchronous on `stream` (a cudaStream_t as an int; 0 is the legacy default
-stream), nothing is kept from one call to the next, and errors raise
+stream, and without one it is torch's current stream), nothing is kept from one call to the next, and errors raise
 PspmlError.
 """
 from __future__ import annotations
@@ -71,6 +71,10 @@ def _index(x: torch.Tensor, dtype, n: int, device: int, what: str) -> int:
     if x.get_device() != device:
         _on(device, x, what)
     return x.data_ptr()
+
+
+def _stream(stream: int | None, device: int) -> int:
+    return torch.cuda.current_stream(device).cuda_stream if stream is None else stream
 
 
 class Rotary:
@@ -140,20 +144,20 @@ def _tokens(x) -> int:
 
 
 def rotary_apply(rotary: Rotary, positions: torch.Tensor, q, q_out, k=None, k_out=None,
-                 stream: int = 0) -> None:
+                 stream: int | None = None) -> None:
     """q_out, k_out = q, k turned to their int32 positions; outputs may be the inputs."""
     n, dev = _tokens(q), rotary.ctx.device
     status = rotary.ctx.lib.pspml_rotary_apply(
         rotary.handle, n, _index(positions, torch.int32, n, dev, "positions"),
         heads(q, dev, "q"), heads(q_out, dev, "q_out", n),
         heads(k, dev, "k", n) if k is not None else None,
-        heads(k_out, dev, "k_out", n) if k_out is not None else None, stream)
+        heads(k_out, dev, "k_out", n) if k_out is not None else None, _stream(stream, dev))
     if status:
         capi.check(status, "pspml_rotary_apply")
 
 
 def rotary_append(rotary: Rotary, positions: torch.Tensor, slots: torch.Tensor, q, q_out, k, v,
-                  cache: KvCache, stream: int = 0) -> None:
+                  cache: KvCache, stream: int | None = None) -> None:
     """q_out = q turned to its positions (q and q_out may be None); token t's turned k and its v
     go to slot slots[t] = page * page_size + slot of the cache (int64; outside it: skipped)."""
     n, dev = _tokens(k), rotary.ctx.device
@@ -163,7 +167,7 @@ def rotary_append(rotary: Rotary, positions: torch.Tensor, slots: torch.Tensor, 
         _index(slots, torch.int64, n, dev, "slots"),
         heads(q, dev, "q", n) if q is not None else None,
         heads(q_out, dev, "q_out", n) if q_out is not None else None,
-        heads(k, dev, "k"), heads(v, dev, "v", n), _ref(cache.view), stream)
+        heads(k, dev, "k"), heads(v, dev, "v", n), _ref(cache.view), _stream(stream, dev))
     if status:
         capi.check(status, "pspml_rotary_append")
 
@@ -177,7 +181,7 @@ def _lse(lse, q, dev) -> int:
 
 
 def prompt(ctx: capi.Context, q, k, v, starts: torch.Tensor, out, lse=None, causal: bool = True,
-           window: int = 0, scale: float | None = None, stream: int = 0) -> None:
+           window: int = 0, scale: float | None = None, stream: int | None = None) -> None:
     """Attention over packed whole prompts: sequence s is tokens starts[s] .. starts[s+1] (int32)
     of q, k, v and out; scale defaults to dim ** -0.5; lse [tokens][heads] float32 or None."""
     dev = ctx.device
@@ -187,14 +191,14 @@ def prompt(ctx: capi.Context, q, k, v, starts: torch.Tensor, out, lse=None, caus
         ctx.handle, _desc(dim, causal, window, scale), n, edges - 1,
         _index(starts, torch.int32, edges, dev, "starts"), heads(q, dev, "q"),
         heads(k, dev, "k", n), heads(v, dev, "v", n), heads(out, dev, "out", n),
-        None if lse is None else _lse(lse, q, dev), stream)
+        None if lse is None else _lse(lse, q, dev), _stream(stream, dev))
     if status:
         capi.check(status, "pspml_attention_prompt")
 
 
 def cached(ctx: capi.Context, q, cache: KvCache, starts: torch.Tensor, lengths: torch.Tensor,
            pages: torch.Tensor, out, max_new: int, lse=None, causal: bool = True, window: int = 0,
-           scale: float | None = None, stream: int = 0) -> None:
+           scale: float | None = None, stream: int | None = None) -> None:
     """Attention of each sequence's new tokens starts[s] .. starts[s+1] of q, at most max_new,
     over its lengths[s] cached keys (the new ones among them), found through row s of the int32
     page table `pages`."""
@@ -211,6 +215,6 @@ def cached(ctx: capi.Context, q, cache: KvCache, starts: torch.Tensor, lengths: 
         _index(starts, torch.int32, seqs + 1, dev, "starts"),
         _index(lengths, torch.int32, seqs, dev, "lengths"), pages.data_ptr(), pages.shape[1],
         heads(q, dev, "q"), _ref(cache.view), heads(out, dev, "out", n),
-        None if lse is None else _lse(lse, q, dev), stream)
+        None if lse is None else _lse(lse, q, dev), _stream(stream, dev))
     if status:
         capi.check(status, "pspml_attention_cached")
