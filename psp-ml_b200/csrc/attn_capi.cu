@@ -1,5 +1,6 @@
 // attn_capi.cu - C entry points of the attention operators: argument checks,
 // rotary frequencies and the choice of kernel.
+#include <algorithm>
 #include <cmath>
 #include <new>
 #include <string>
@@ -94,7 +95,8 @@ int check_rotary_desc(const pspml_rotary_desc* d) {
   if (d->layout != PSPML_ROTARY_HALF && d->layout != PSPML_ROTARY_INTERLEAVED)
     return bad("rotary: unknown layout");
   if (!(d->base > 0.0) || !std::isfinite(d->base)) return bad("rotary: base must be positive");
-  if (!std::isfinite(d->amplitude)) return bad("rotary: amplitude must be finite");
+  if (!std::isfinite(static_cast<float>(d->amplitude)))  // the kernels' type
+    return bad("rotary: amplitude must be finite");
   if (d->scaling < PSPML_ROTARY_SCALE_NONE || d->scaling > PSPML_ROTARY_SCALE_PARTS)
     return bad("rotary: unknown scaling");
   if (d->scaling != PSPML_ROTARY_SCALE_NONE && (!(d->factor > 0.0) || !std::isfinite(d->factor)))
@@ -108,7 +110,8 @@ int check_rotary_desc(const pspml_rotary_desc* d) {
   return PSPML_OK;
 }
 
-void frequencies(const pspml_rotary_desc& d, unsigned long long* out) {
+// False if a frequency is not finite: a base or factor too small for doubles.
+bool frequencies(const pspml_rotary_desc& d, unsigned long long* out) {
   const double two_pi = 6.283185307179586476925286766559;
   double base = d.base;
   if (d.scaling == PSPML_ROTARY_SCALE_BASE)
@@ -121,12 +124,14 @@ void frequencies(const pspml_rotary_desc& d, unsigned long long* out) {
       const double keep = std::fmin(1.0, std::fmax(0.0, (r - d.low) / (d.high - d.low)));
       f = keep * f + (1.0 - keep) * f / d.factor;
     }
+    if (!std::isfinite(f)) return false;
     double turns = f / two_pi;
     turns -= std::floor(turns);
     // turns < 1 has 53 bits: the product with 2^64 is exact but may round up
     // to a whole turn only if turns did, which floor excludes.
     out[i] = static_cast<unsigned long long>(std::ldexp(turns, 64));
   }
+  return true;
 }
 
 RotaryView view_of(const pspml_heads* in, const pspml_heads* out) {
@@ -310,8 +315,9 @@ int pspml_rotary_frequencies(const pspml_rotary_desc* d, uint64_t* host_out) {
   int st = check_rotary_desc(d);
   if (st) return st;
   if (host_out == nullptr && d->rot_dim > 0) return bad("null output");
-  static_assert(sizeof(uint64_t) == sizeof(unsigned long long), "64-bit fractions");
-  frequencies(*d, reinterpret_cast<unsigned long long*>(host_out));
+  unsigned long long f[kMaxRotaryDim / 2];
+  if (!frequencies(*d, f)) return bad("rotary: a frequency is not finite");
+  std::copy_n(f, d->rot_dim / 2, host_out);
   return PSPML_OK;
 }
 
@@ -322,16 +328,16 @@ int pspml_rotary_create(pspml_ctx* ctx, const pspml_rotary_desc* d, pspml_rotary
   if (ctx == nullptr) return bad("null context");
   int st = check_rotary_desc(d);
   if (st) return st;
+  unsigned long long f[kMaxRotaryDim / 2];
+  if (!frequencies(*d, f)) return bad("rotary: a frequency is not finite");
   if ((st = cuda_status(cudaSetDevice(ctx->device), "cudaSetDevice"))) return st;
   auto* r = new (std::nothrow) pspml_rotary();
   if (r == nullptr) return set_error(PSPML_ERR_OOM, "host allocation failed");
   r->device = ctx->device;
   r->num_sms = ctx->num_sms;
   r->d = *d;
-  unsigned long long f[kMaxRotaryDim / 2];
   const size_t bytes = d->rot_dim / 2 * sizeof(f[0]);
   if (bytes > 0) {
-    frequencies(*d, f);
     st = cuda_status(cudaMalloc(&r->freq, bytes), "cudaMalloc(rotary)");
     // Uploaded on the context's stream and waited for: calls on any stream
     // may follow.
