@@ -28,6 +28,14 @@ int dtype_bytes(int32_t t) {
   }
 }
 
+// Index and log-sum-exp arrays are read and written as whole elements.
+template <typename T>
+int check_array(const T* p, const char* name) {
+  return reinterpret_cast<uintptr_t>(p) % sizeof(T) == 0
+             ? PSPML_OK
+             : bad(std::string(name) + ": not aligned to its element size");
+}
+
 // A view's own consistency.  Output views also have to give every element
 // an address of its own.
 int check_heads(const pspml_heads* h, const char* name, int64_t tokens, bool output) {
@@ -193,7 +201,7 @@ void fill_rotary(const pspml_rotary* r, int64_t tokens, const int32_t* positions
 
 int check_attention(const pspml_ctx* ctx, const pspml_attention_desc* d, int64_t tokens,
                     int32_t sequences, const int32_t* starts, const pspml_heads* q,
-                    const pspml_heads* out) {
+                    const pspml_heads* out, const float* lse) {
   if (ctx == nullptr) return bad("null context");
   if (d == nullptr) return bad("null attention descriptor");
   if (!std::isfinite(d->scale)) return bad("attention: scale must be finite");
@@ -204,8 +212,10 @@ int check_attention(const pspml_ctx* ctx, const pspml_attention_desc* d, int64_t
   if (tokens < 0 || tokens > INT32_MAX) return bad("attention: tokens must be 0 .. 2^31 - 1");
   if (sequences < 0) return bad("attention: negative number of sequences");
   if (starts == nullptr && sequences > 0) return bad("attention: null starts");
-  int st = check_heads(q, "q", tokens, false);
+  int st = check_array(starts, "starts");
   if (st) return st;
+  if ((st = check_array(lse, "lse"))) return st;
+  if ((st = check_heads(q, "q", tokens, false))) return st;
   if ((st = check_heads(out, "out", tokens, true))) return st;
   if (q->dtype == PSPML_DTYPE_S8) return bad("q: S8 is not an attention input type");
   if (q->head_dim > kMaxHeadDim)
@@ -372,8 +382,9 @@ int pspml_rotary_apply(pspml_rotary* r, int64_t tokens, const int32_t* positions
   if (positions == nullptr && tokens > 0) return bad("null positions");
   if ((k == nullptr) != (k_out == nullptr)) return bad("k and k_out go together");
   if (q_out == nullptr) return bad("null q output");
-  int st = check_rotary_pair(r, q, q_out, tokens, "q");
+  int st = check_array(positions, "positions");
   if (st) return st;
+  if ((st = check_rotary_pair(r, q, q_out, tokens, "q"))) return st;
   if (k != nullptr) {
     if ((st = check_rotary_pair(r, k, k_out, tokens, "k")) || (st = same_quant(q, k, "q and k")))
       return st;
@@ -399,8 +410,10 @@ int pspml_rotary_append(pspml_rotary* r, int64_t tokens, const int32_t* position
   if ((positions == nullptr || slots == nullptr) && tokens > 0)
     return bad("null positions or slots");
   if ((q == nullptr) != (q_out == nullptr)) return bad("q and q_out go together");
-  int st = check_cache(cache, true);
+  int st = check_array(positions, "positions");
   if (st) return st;
+  if ((st = check_array(slots, "slots"))) return st;
+  if ((st = check_cache(cache, true))) return st;
   if ((st = check_rotary_pair(r, k, nullptr, tokens, "k"))) return st;
   if ((st = check_rotary_pair(r, v, nullptr, tokens, "v"))) return st;
   if ((st = same_quant(k, v, "k and v"))) return st;
@@ -435,7 +448,7 @@ int pspml_attention_prompt(pspml_ctx* ctx, const pspml_attention_desc* d, int64_
                            const pspml_heads* k, const pspml_heads* v, const pspml_heads* out,
                            float* lse, void* stream) {
   clear_error();
-  int st = check_attention(ctx, d, tokens, sequences, starts, q, out);
+  int st = check_attention(ctx, d, tokens, sequences, starts, q, out, lse);
   if (st) return st;
   if ((st = check_heads(k, "k", tokens, false)) || (st = check_heads(v, "v", tokens, false)))
     return st;
@@ -463,13 +476,14 @@ int pspml_attention_cached(pspml_ctx* ctx, const pspml_attention_desc* d, int64_
                            const pspml_heads* q, const pspml_kv_cache* cache,
                            const pspml_heads* out, float* lse, void* stream) {
   clear_error();
-  int st = check_attention(ctx, d, tokens, sequences, starts, q, out);
+  int st = check_attention(ctx, d, tokens, sequences, starts, q, out, lse);
   if (st) return st;
   if ((st = check_cache(cache, false))) return st;
   if (max_new < 0) return bad("negative max_new");
   if (pages_stride < 0) return bad("negative pages_stride");
   if (sequences > 0 && (lengths == nullptr || (pages == nullptr && pages_stride > 0)))
     return bad("null lengths or pages");
+  if ((st = check_array(lengths, "lengths")) || (st = check_array(pages, "pages"))) return st;
   if (cache->dtype != q->dtype) return bad("q and the cache: types differ");
   if (cache->head_dim != q->head_dim || q->heads % cache->heads != 0)
     return bad("q and the cache: shapes do not go together");
