@@ -395,7 +395,9 @@ typedef struct pspml_rotary pspml_rotary;
 
 /* Writes the rot_dim/2 frequencies to host memory, in turns per position as
  * 64-bit binary fractions (f_i / 2pi * 2^64, modulo a turn): a position
- * times a frequency wraps exactly, so angles lose nothing at any position.
+ * times a frequency wraps without rounding, so an angle is off by no more
+ * than the position times the frequency's own error (a double's, 2^-53 of
+ * it; 2^-24 of a turn for the fastest pair at position 2^31).
  * Needs no device. */
 int pspml_rotary_frequencies(const pspml_rotary_desc* d, uint64_t* host_out);
 /* A rotation kept on the context's device; it may outlive the context. */

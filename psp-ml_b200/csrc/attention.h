@@ -91,6 +91,13 @@ template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, f
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
+// 2^x as the special function unit gives it (2^-22 relative).
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 // The int8 an output value is stored as: nearest (ties to even), clamped
 // while still a float so that infinities saturate; NaN gives the zero point.
 __device__ __forceinline__ int8_t quantise_s8(float v, float inv_scale, int32_t zero) {

@@ -29,10 +29,11 @@
 //
 // A CTA stays for many items (a pair of tiles and a key head): the next one's
 // loads and first scores run while this one ends.  Many items are handed out
-// by a counter, those with the most keys first.  Few items are cut: the list
-// of all their key tiles is divided into equal shares, and where a share cuts
-// an item the pieces go to the workspace, unnormalised, and the CTA that
-// arrives last joins them in order, so the same call gives the same bits.
+// by a counter, within a sequence those with the most keys first.  Few items
+// are cut: the list of all their key tiles is divided into equal shares, and
+// where a share cuts an item the pieces go to the workspace, unnormalised, and
+// the CTA that arrives last joins them in order, so the same call gives the
+// same bits.
 //
 // What bounds it: the chain of one tile (scores 592 clocks and 270 until they
 // are seen, softmax 2000 to 2250, the last half of P V and its completion 470)
@@ -71,7 +72,6 @@ constexpr int kPieces = 2;        // in which P is handed to the MMA warp
 // tiles 189 us whole and 131 us cut.
 constexpr int kItemsPerSm = 2;
 constexpr int kCutTiles = 6;
-constexpr int kCountedSequences = 4096;
 constexpr float kGrowLog2 = 8.0f; // largest stale maximum, as a power of two
 
 struct TcArgs {
@@ -95,16 +95,10 @@ struct TcShape {
   static constexpr int kTileBytes = 128 * DP * 2;   // Q tile, K or V slot
   static constexpr int kSlots = DP == 128 ? 5 : 8;
   static constexpr int kSmem = 1024 + (2 + kSlots) * kTileBytes;
-  static constexpr uint32_t kCols = DP == 128 ? 512 : 512;
+  static constexpr uint32_t kCols = 512;
   static constexpr uint32_t kS = 0;                 // S/P of A, then of B
   static constexpr uint32_t kO = 256;               // O of A, then of B
 };
-
-__device__ __forceinline__ float tc_ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 
 // Two floats in one 64-bit register, and the packed arithmetic on them.
 __device__ __forceinline__ uint64_t f2(float lo, float hi) {
@@ -404,8 +398,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     tmem_alloc(&tmem_slot, Sh::kCols);
     tmem_relinquish();
   }
-  // Few items: their key tiles are counted, with room for the tiles as
-  // scratch.  Cutting pays where one item outlasts an equal share by more
+  // Few items, so fewer sequences and pairs than kItemsPerSm an SM (some 11000
+  // pairs if `starts` decreases against its contract, 44 KB): their key tiles
+  // are counted, with room for the tiles as scratch.  Cutting pays where one item outlasts an equal share by more
   // than the pieces cost.
   TcShare share;
   bool more = p.items > gridDim.x;  // than one item a CTA, handed out by the counter
@@ -871,7 +866,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         const float m2 = fmaxf(m, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])));
         const bool grow = (m2 - m) * p.scale_log2 > kGrowLog2;
         if (__any_sync(~0u, grow)) {
-          const float f = grow ? tc_ex2((m - m2) * p.scale_log2) : 1.0f;
+          const float f = grow ? ex2((m - m2) * p.scale_log2) : 1.0f;
           if (grow) m = m2;
           l *= f;
           if (i > 0) {
@@ -896,8 +891,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             const uint32_t* q = s + 32 * c + 2 * x;
             float e0, e1;
             f2_get(f2_fma(f2(__uint_as_float(q[0]), __uint_as_float(q[1])), scale2, base2), e0, e1);
-            e0 = tc_ex2(e0);
-            e1 = tc_ex2(e1);
+            e0 = ex2(e0);
+            e1 = ex2(e1);
             sums[x & 1] = f2_add(sums[x & 1], f2(e0, e1));
             w[x] = pack2<T>(e0, e1);
           }
@@ -996,7 +991,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
               const float2 ml = __ldcg(p.part_ml + slot_of(x) * 256 + tid);
               const float top = fmaxf(mm, ml.x);
               const float bs = top == -INFINITY ? 0.0f : top;
-              sum = sum * tc_ex2(mm - bs) + ml.y * tc_ex2(ml.x - bs);
+              sum = sum * ex2(mm - bs) + ml.y * ex2(ml.x - bs);
               mm = top;
             }
             const float bs = mm == -INFINITY ? 0.0f : mm;
@@ -1013,7 +1008,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 #pragma unroll 4
               for (int x = 0; x < pieces; ++x) {
                 const float2 ml = __ldcg(p.part_ml + slot_of(x) * 256 + tid);
-                const float f = tc_ex2(ml.x - bs);
+                const float f = ex2(ml.x - bs);
                 float4 v[kCols / 4];
 #pragma unroll
                 for (int y = 0; y < kCols / 4; ++y)
@@ -1164,7 +1159,7 @@ cudaError_t launch_attn_tc(const AttnArgs& a, const AttnWork& w, cudaStream_t s)
   const int64_t most_keys = a.paged ? a.pages_stride * a.page_size : a.tokens;
   int64_t grid = std::min<int64_t>(w.num_sms, kAttnCounters - 2);
   p.shares = p.items < static_cast<int64_t>(kItemsPerSm) * grid &&
-             a.sequences <= kCountedSequences && most_keys > kCutTiles * kKeys &&
+             most_keys > kCutTiles * kKeys &&
              most_keys < (1 << 28);  // the count stays within 32 bits
   if (p.shares) {
     grid = std::min(grid, p.items * ((most_keys + kMinShare * kKeys - 1) / (kMinShare * kKeys)));

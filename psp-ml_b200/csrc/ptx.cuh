@@ -365,10 +365,9 @@ __host__ __device__ constexpr uint32_t make_idesc_f16(int m, int n, int fmt, int
          | (static_cast<uint32_t>(m >> 4) << 24);    // M >> 4
 }
 
-// 128 columns of this warp's 32 lanes.  Loads and wait are one statement:
-// until the wait the registers are the hardware's, and the copies that a
-// wait of its own with the registers as operands brings with it would read
-// them too early and let what lands overwrite whatever has taken their place.
+// 128 columns of this warp's 32 lanes.  Loads and wait are one statement, so
+// that the compiler can place nothing between them that touches registers
+// whose values have not landed yet.
 __device__ __forceinline__ void tmem_ld128(uint32_t taddr, uint32_t (&r)[128]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x32.b32 {"

@@ -4,9 +4,10 @@
 // Pair (x, y) i of a head at position p turns by the angle p * f_i:
 //   x' = amp * (x cos - y sin),  y' = amp * (x sin + y cos).
 // f_i is held in turns per position as a 64-bit binary fraction, so p * f_i
-// modulo one turn is one wrapping integer product: the angle is exact to
-// 2^-64 turns per position however long the context, where a 32-bit float
-// product would be off by 6e-3 rad at position 100000.  Only the reduced
+// modulo one turn is one wrapping integer product, in which nothing is lost:
+// the angle is as good as the frequency, a double's quotient (about 2^-53 of
+// itself), times the position, 2^-24 turns for the fastest pair at position
+// 2^31.  A 32-bit float product would be off by 6e-3 rad at position 100000.  Only the reduced
 // angle is rounded to a float; sums and products are 32-bit and rounded once
 // to the output type.
 //

@@ -160,6 +160,25 @@ def test_rows_past_max_new_hold_nan(ctx, at, window, computed, lengths, new, hq,
         a += m
 
 
+@pytest.mark.parametrize("bound", [4, 80])
+@pytest.mark.parametrize("lengths,new,hq,hkv,dim,dtype", [
+    ([20000], [4], 4, 1, 128, BF16), ([7000, 30], [3, 4], 8, 2, 80, F16)])
+def test_cached_not_causal_cut(ctx, at, bound, lengths, new, hq, hkv, dim, dtype):
+    # Cut over the device, every row seeing all keys, those of the rows after it too.
+    keys = [_rand(40 + s, n, hkv, dim, dtype=dtype) for s, n in enumerate(lengths)]
+    values = [_rand(44 + s, n, hkv, dim, dtype=dtype) for s, n in enumerate(lengths)]
+    cache, n, table = _cache(at, keys, values, 16)
+    q = _rand(48, sum(new), hq, dim, dtype=dtype)
+    out, lse = torch.zeros_like(q), torch.zeros((sum(new), hq), device="cuda")
+    at.cached(ctx, q, cache, _starts(new), n, table, out, bound, lse=lse, causal=False)
+    ctx.check_device()
+    a, parts = 0, []
+    for s, m in enumerate(new):
+        parts.append(ref.attend(q[a:a + m], keys[s], values[s], lengths[s] - m, False, 0, dim ** -0.5))
+        a += m
+    _same(out, lse, tuple(torch.cat(x) for x in zip(*parts)))
+
+
 @pytest.mark.parametrize("tokens,hq,hkv,dim,dtype", [(700, 8, 2, 128, BF16), (2600, 1, 1, 64, F16)])
 def test_rows_done_again_stay(ctx, at, tokens, hq, hkv, dim, dtype):
     # Other lanes of the warp write a row done again than wrote it first: every time the second
