@@ -132,7 +132,9 @@ int pspml_ctx_set_timeout_ms(pspml_ctx* ctx, int64_t timeout_ms);
 /* Reads and clears the device-side error word that kernels set when a
  * bounded wait expires; returns PSPML_ERR_DEVICE_WAIT if it was set.  The
  * tensor-core kernels bound every wait at 4 s; on expiry they record a code
- * here, stop, let issued copies land, free tensor memory and return. */
+ * here, stop, let issued copies land, free tensor memory and return.  When
+ * the word was set, the call waits for everything on the device; outputs of
+ * the context's calls up to then are not to be trusted. */
 int pspml_ctx_check_device(pspml_ctx* ctx);
 /* Diagnostic of the path above (no counterpart in the reference): one
  * thread waits, with the kernels' bounded wait, on a barrier that it
@@ -427,7 +429,8 @@ int pspml_rotary_append(pspml_rotary* r, int64_t tokens, const int32_t* position
  * holds: keys past a sequence's end, masked keys, other sequences.  Values
  * that are not finite cost time there: the rows that share a tile with them
  * are computed again on CUDA cores (16384 tokens of 32 heads with one bad
- * token near the end: 50 ms instead of 1.7; 5 s after a million keys). */
+ * token near the end: 51 ms instead of 1.7, with an infinity in one column
+ * of all of them 0.5 s; a bad value after a million keys: 5 s). */
 typedef struct pspml_attention_desc {
   float scale;
   int32_t causal;        /* 0 / 1                                           */

@@ -14,11 +14,14 @@
 //   2. eight rows at a time: a lane holds a few columns of all eight, and each
 //      key is read once; a row's score is summed over the lanes and kept by
 //      four of them, and values of keys that a row does not see are skipped.
+// Infinities that a row does see count with the weight that the tile used: one
+// that rounds to 0 in the operands' type (below 2^-25 in F16) makes NaN of them.
 // Finite outputs never come here.  One bad token costs the rows of the tokens
 // that share its tile one more pass over their keys, at most 127 tokens' of a
-// prompt, bound by latency on few warps: 16384 tokens of 32 heads take 50 ms
-// with token 12127 bad, 3 ms with token 100 or all of them bad, 1.7 ms with
-// none.  Sums and statistics are 32-bit, weights are not rounded.
+// prompt, bound by latency on few warps: 16384 tokens of 32 heads take 51 ms
+// with token 12127 bad, 3 ms with token 100 or all of them NaN, 0.5 s with an
+// infinity in one column of all of them (no row is settled), 1.7 ms with none
+// bad.  Sums and statistics are 32-bit, weights are not rounded.
 #pragma once
 
 #include <cmath>

@@ -39,9 +39,10 @@
 // are seen, softmax 2000 to 2250, the last half of P V and its completion 470)
 // sets 3430 clocks a pair of key tiles against 2208 of tensor work; shared
 // memory feeds the scores at its full 128 bytes a clock.  On a B200, BF16, 32
-// query and 8 key heads of 128: 16384 tokens 1.72 ms alone (1.28 PFLOP/s) and
-// 2.01 ms in a long row of passes, where power limits the clock; 17 packed
-// prompts of up to 2048 tokens 140 us (0.74 PFLOP/s).
+// query and 8 key heads of 128: 16384 tokens 1.73 ms alone (1.27 PFLOP/s) and
+// 2.00 ms in a long row of passes, where power limits the clock; 17 packed
+// prompts of up to 2048 tokens 148 us (0.70 PFLOP/s), 135 us with inputs that
+// stay in L2.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -470,7 +471,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         closed = item_close(&book, it);
         if (closed) tc_fail(p.err, state, kDevErrEpiWait);
       }
-      if (__any_sync(~0u, closed)) return nullptr;
+      closed = __any_sync(~0u, closed);
+      __syncwarp();  // the record, if it is there, is there for every lane
+      if (closed) return nullptr;
     }
     return &items[it & 1];
   };
